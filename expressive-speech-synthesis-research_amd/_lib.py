@@ -10,7 +10,7 @@ import os
 _PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG, 'libestts.so')
 
-ABI_VERSION = 36
+ABI_VERSION = 37
 ACT_NONE, ACT_RELU, ACT_TANH = 0, 1, 2
 ACT = {None: ACT_NONE, 'linear': ACT_NONE, 'none': ACT_NONE, 'relu': ACT_RELU, 'tanh': ACT_TANH}
 
@@ -118,6 +118,25 @@ class PrenetRowArgs(C.Structure):
                 ('out', _vp), ('ldo', _i32), ('M', _i32)]
 
 
+class PagePlanArgs(C.Structure):
+    _fields_ = [('lengths', _vp), ('n_new', _vp), ('block_table', _vp), ('ld_table', _i64), ('free_pages', _vp), ('n_free', _vp),
+                ('slots', _vp), ('positions', _vp), ('lengths_out', _vp), ('n_free_out', _vp), ('refused', _vp), ('ws', _vp),
+                ('B', _i32), ('P', _i32), ('n_pages', _i32), ('page', _i32), ('T', _i32), ('R', _i32)]
+
+
+class PageWriteArgs(C.Structure):
+    _fields_ = [('k', _vp), ('ldk', _i64), ('v', _vp), ('ldv', _i64), ('k_cache', _vp), ('v_cache', _vp), ('s_page', _i64), ('s_head', _i64),
+                ('s_row', _i64), ('slots', _vp), ('T', _i32), ('heads', _i32), ('depth', _i32), ('page', _i32), ('n_pages', _i32),
+                ('type', _i32)]
+
+
+class PagedAttentionArgs(C.Structure):
+    _fields_ = [('q', _vp), ('ldq', _i64), ('k_cache', _vp), ('v_cache', _vp), ('s_page', _i64), ('s_head', _i64), ('s_row', _i64),
+                ('block_table', _vp), ('ld_table', _i64), ('lengths', _vp), ('key_mask', _vp), ('mask_sb', _i64), ('mask_ss', _i64),
+                ('ctx', _vp), ('ldo', _i64), ('scale', _f32), ('B', _i32), ('H', _i32), ('kv_heads', _i32), ('depth', _i32), ('page', _i32),
+                ('n_pages', _i32), ('P', _i32), ('max_len', _i32), ('type', _i32), ('ws', _vp), ('ws_bytes', _i64)]
+
+
 class ProgOp(C.Structure):
     _fields_ = [('kind', _i32), ('n_patch', _i32), ('args', _vp), ('patch_offset', _i32 * PROG_MAX_PATCH),
                 ('patch_is_ptr', _i32 * PROG_MAX_PATCH), ('patch_stride', _i64 * PROG_MAX_PATCH)]
@@ -196,6 +215,10 @@ SIGNATURES = {
     'estts_cross_attention_row': (_i32, [C.POINTER(CrossRowArgs), _vp]),
     'estts_decoder_block_row': (_i32, [C.POINTER(DecoderBlockArgs), _vp]),
     'estts_prenet_row': (_i32, [C.POINTER(PrenetRowArgs), _vp]),
+    'estts_page_plan': (_i32, [C.POINTER(PagePlanArgs), _vp]),
+    'estts_page_write': (_i32, [C.POINTER(PageWriteArgs), _vp]),
+    'estts_paged_attention': (_i32, [C.POINTER(PagedAttentionArgs), _vp]),
+    'estts_paged_attention_ws_bytes': (_i64, [_i32, _i32, _i32, _i32, _i32, _i32]),
     'estts_masked_mae': (_i32, [_vp, _i32, _vp, _i32, _vp, _i32, _i32, _vp]),
     'estts_wavernn_prep': (_i32, [C.POINTER(WavernnPrepArgs), _vp]),
     'estts_gru_gates': (_i32, [_vp, _i32, _vp, _i32, _vp, _i32, _vp, _i32, _vp, _i32, _i32, _i32, _vp]),

@@ -468,13 +468,17 @@ extern "C" int estts_run_program(const estts_prog_op* ops, int32_t n_ops, int32_
         estts_cross_row_args c;
         estts_decoder_block_args d;
         estts_prenet_row_args p;
+        estts_page_plan_args pp;
+        estts_page_write_args pw;
+        estts_paged_attention_args pa;
     } blk;
-    static const size_t sizes[7] = {sizeof(estts_gemm_args), sizeof(estts_attention_args), sizeof(estts_rownorm_args),
+    static const size_t sizes[10] = {sizeof(estts_gemm_args), sizeof(estts_attention_args), sizeof(estts_rownorm_args),
                                     sizeof(estts_rowmask_args), sizeof(estts_cross_row_args), sizeof(estts_decoder_block_args),
-                                    sizeof(estts_prenet_row_args)};
+                                    sizeof(estts_prenet_row_args), sizeof(estts_page_plan_args), sizeof(estts_page_write_args),
+                                    sizeof(estts_paged_attention_args)};
     for (int i = 0; i < n_ops; ++i) {
         const estts_prog_op& op = ops[i];
-        ESTTS_CHECK_ARG(op.kind >= 0 && op.kind < 7 && op.args && op.n_patch >= 0 && op.n_patch <= ESTTS_PROG_MAX_PATCH,
+        ESTTS_CHECK_ARG(op.kind >= 0 && op.kind < 10 && op.args && op.n_patch >= 0 && op.n_patch <= ESTTS_PROG_MAX_PATCH,
                         "estts_run_program: op %d is malformed", i);
         memcpy(&blk, op.args, sizes[op.kind]);
         char* base = reinterpret_cast<char*>(&blk);
@@ -501,6 +505,9 @@ extern "C" int estts_run_program(const estts_prog_op* ops, int32_t n_ops, int32_
             case 4: rc = estts_cross_attention_row(&blk.c, stream); break;
             case 5: rc = estts_decoder_block_row(&blk.d, stream); break;
             case 6: rc = estts_prenet_row(&blk.p, stream); break;
+            case 7: rc = estts_page_plan(&blk.pp, stream); break;
+            case 8: rc = estts_page_write(&blk.pw, stream); break;
+            case 9: rc = estts_paged_attention(&blk.pa, stream); break;
             default: rc = estts_row_zero_mask(blk.m.x, blk.m.ldx, blk.m.mask, blk.m.M, blk.m.D, stream); break;
         }
         if (rc != 0) return rc;

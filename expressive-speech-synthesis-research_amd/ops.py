@@ -92,24 +92,42 @@ def _record(kind, info, fn, *args, keep=()):
 _program = None
 
 
+_program_scratch = None        # [buffers of the program being recorded, how many this recording has used]
+
+
+def _scratch(nbytes, device):
+    """Scratch of one launch: it goes back to the allocator with the call, which hands it to later work of this stream only (to a
+    graph of its own under capture); a step program's launches keep theirs, the same in both recordings."""
+    if _program_scratch is None:
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
+    bufs, k = _program_scratch
+    _program_scratch[1] = k + 1
+    if k == len(bufs):
+        bufs.append(torch.empty(nbytes, dtype=torch.uint8, device=device))
+    if bufs[k].numel() != nbytes:
+        raise RuntimeError('StepProgram: steps 0 and 1 issue launches of different sizes')
+    return bufs[k]
+
+
 class StepProgram:
     """A fixed sequence of launches whose arguments depend affinely on a step index, issued from one C call per step
     (estts_run_program).  Built by recording the same Python code for step 0 and step 1: every argument field that
     differs between the two recordings becomes a patch `field += step * (value1 - value0)`."""
 
-    KINDS = {'gemm': 0, 'attention': 1, 'rownorm': 2, 'row_zero_mask': 3, 'cross_attention_row': 4, 'decoder_block_row': 5, 'prenet_row': 6}
+    KINDS = {'gemm': 0, 'attention': 1, 'rownorm': 2, 'row_zero_mask': 3, 'cross_attention_row': 4, 'decoder_block_row': 5, 'prenet_row': 6,
+             'page_plan': 7, 'page_write': 8, 'paged_attention': 9}
 
     def __init__(self, record_step):
         """record_step(i): issues the launches of step i through this module's op functions."""
-        global _program
-        recs = []
+        global _program, _program_scratch
+        recs, scratch = [], []
         for i in (0, 1):
-            _program = []
+            _program, _program_scratch = [], [scratch, 0]
             try:
                 record_step(i)
             finally:
                 recs.append(_program)
-                _program = None
+                _program = _program_scratch = None
         r0, r1 = recs
         if len(r0) != len(r1) or any(a[0] != b[0] for a, b in zip(r0, r1)):
             raise RuntimeError('StepProgram: steps 0 and 1 issue different launch sequences')
@@ -608,6 +626,169 @@ def decoder_block_row(wqkv, wos, sa_ln, sa_last_ln, wqc, woc, ca_ln, wff, cache,
                                   'bytes': 4.0 * (8 * d * d + 2 * (Lk + pos + 1) * d) + 4.0 * (6 * d + 4 * Lk)},
             _lib.load().estts_decoder_block_row, a, keep=a._keep)
     return y2
+
+
+KV_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}     # ESTTS_KV_*
+
+
+def _check_here(what, **tensors):
+    """All tensors on the current device, to whose current stream launches go (None aside)."""
+    for name, t in tensors.items():
+        if t is not None and (not t.is_cuda or t.get_device() != torch.cuda.current_device()):
+            raise ValueError(f'{what}: {name} is on {t.device}, which is not the current device')
+
+
+def _check_rows(what, t, name, rows, width):
+    if t.dtype != torch.float32:
+        raise TypeError(f'{what}: {name} must be float32, got {t.dtype}')
+    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] < width or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise ValueError(f'{what}: {name} must be [{rows}, >= {width}] with contiguous rows, got {list(t.shape)} with strides {t.stride()}')
+    return t.stride(0) if rows > 1 else width
+
+
+def _check_i32(what, t, name, shape):
+    if t.dtype != torch.int32:
+        raise TypeError(f'{what}: {name} must be int32, got {t.dtype}')
+    if tuple(t.shape) != shape or not t.is_contiguous():
+        raise ValueError(f'{what}: {name} must be a contiguous {list(shape)} tensor, got {list(t.shape)} with strides {t.stride()}')
+
+
+def _check_table(what, block_table, B):
+    if block_table.dtype != torch.int32:
+        raise TypeError(f'{what}: block_table must be int32, got {block_table.dtype}')
+    if block_table.dim() != 2 or block_table.shape[0] != B or block_table.shape[1] < 1 or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
+        raise ValueError(f'{what}: block_table must be [{B}, pages of a request] with contiguous rows, got {list(block_table.shape)}')
+    return block_table.stride(0) if B > 1 else block_table.shape[1]
+
+
+def _page_strides(t):
+    """Element strides of page, head and row of a cache; those of dimensions of size 1, which nothing is multiplied with, as 0 / depth."""
+    n, (p, h, r, _) = t.shape, t.stride()
+    return p if n[0] > 1 else 0, h if n[1] > 1 else 0, r if n[2] > 1 else n[3]
+
+
+def _check_pages(what, k_cache, v_cache):
+    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape or v_cache.dtype != k_cache.dtype or _page_strides(v_cache) != _page_strides(k_cache):
+        raise ValueError(f'{what}: k_cache and v_cache must be [n_pages, kv_heads, page, depth] tensors of the same strides and type')
+    if k_cache.dtype not in KV_TYPES:
+        raise TypeError(f'{what}: caches hold float32, bfloat16 or float16, got {k_cache.dtype}')
+    if k_cache.stride(3) != 1 or v_cache.stride(3) != 1:
+        raise ValueError(f'{what}: the last dimension of the caches must be contiguous')
+    return _page_strides(k_cache)
+
+
+def new_paged_cache(n_pages, page, kv_heads, depth, dtype=torch.float32, device='cuda'):
+    """(k_cache, v_cache) of n_pages pages of `page` rows (a multiple of 16) each, for page_write / paged_attention."""
+    return tuple(torch.zeros(n_pages, kv_heads, page, depth, dtype=dtype, device=device) for _ in range(2))
+
+
+def page_plan(lengths, new, block_table, free_pages, n_free, page, slots, positions=None, lengths_out=None, n_free_out=None, refused=None):
+    """The page plan of a step (estts_page_plan): request b has lengths[b] rows in its pages and new[b] more are about to come
+    (-1: it has ended and gives its pages back).  The requests that fit take the pages they need off the stack free_pages
+    [n_pages] (n_free [1] entries) into block_table [B, P]; slots says where each new row goes: [T], the rows of all requests packed
+    one after another, or [B, R], request b's rows at [b, :new[b]]; -1 where there is no row or the request was turned away.
+    positions: like slots, the place of each row in its request.  lengths and n_free are updated in place unless lengths_out /
+    n_free_out are given; refused [1] counts the requests that were turned away (their length stays).  All int32; nothing
+    is read back by the host, so a captured step plans itself anew on every replay."""
+    B = lengths.numel()
+    lengths_out = lengths if lengths_out is None else lengths_out
+    n_free_out = n_free if n_free_out is None else n_free_out
+    for t, n, shape in ((lengths, 'lengths', (B,)), (new, 'new', (B,)), (free_pages, 'free_pages', (free_pages.numel(),)), (n_free, 'n_free', (1,)),
+                        (lengths_out, 'lengths_out', (B,)), (n_free_out, 'n_free_out', (1,)), (slots, 'slots', tuple(slots.shape))):
+        _check_i32('page_plan', t, n, shape)
+    if positions is not None:
+        _check_i32('page_plan', positions, 'positions', tuple(slots.shape))
+    if refused is not None:
+        _check_i32('page_plan', refused, 'refused', (1,))
+    ld = _check_table('page_plan', block_table, B)
+    if slots.dim() not in (1, 2) or (slots.dim() == 2 and slots.shape[0] != B):
+        raise ValueError(f'page_plan: slots must be [T] (packed rows) or [{B}, R] (padded rows), got {list(slots.shape)}')
+    _check_here('page_plan', lengths=lengths, new=new, block_table=block_table, free_pages=free_pages, n_free=n_free, slots=slots, positions=positions,
+                lengths_out=lengths_out, n_free_out=n_free_out, refused=refused)
+    ws = _scratch(12 * B, lengths.device)
+    a = _lib.PagePlanArgs(lengths.data_ptr(), new.data_ptr(), block_table.data_ptr(), ld, free_pages.data_ptr(), n_free.data_ptr(), slots.data_ptr(),
+                          _ptr(positions), lengths_out.data_ptr(), n_free_out.data_ptr(), _ptr(refused), ws.data_ptr(),
+                          B, block_table.shape[1], free_pages.numel(), page, slots.numel(), slots.shape[1] if slots.dim() == 2 else 0)
+    keep = (lengths, new, block_table, free_pages, n_free, slots, positions, lengths_out, n_free_out, refused, ws)
+    if _program is not None:
+        _program.append(('page_plan', a, keep))
+        return slots
+    check(_lib.load().estts_page_plan(a, _stream()), 'estts_page_plan')
+    if _trace is not None or _debug_sync:
+        _record('page_plan', {'B': B, 'T': slots.numel(), 'page': page, 'flops': 0.0, 'bytes': 4.0 * (3 * B + 2 * slots.numel())},
+                _lib.load().estts_page_plan, a, keep=keep)
+    return slots
+
+
+def page_write(k, v, k_cache, v_cache, slots):
+    """Rows k, v ([T, >= kv_heads * depth] float32 views, head after head) into the pages (estts_page_write): row t goes to slots[t]
+    (int32, any shape with T elements; page * page size + row, what page_plan writes), rounded to the caches' type; rows with a
+    slot outside the cache go nowhere.  The slots of a call must be distinct."""
+    s_page, s_head, s_row = _check_pages('page_write', k_cache, v_cache)
+    n_pages, Hk, page, D = k_cache.shape
+    if (n_pages > 1 and not s_page) or (Hk > 1 and not s_head) or not s_row:
+        raise ValueError('page_write: the caches must not be broadcast views')
+    T = slots.numel()
+    _check_i32('page_write', slots, 'slots', tuple(slots.shape))
+    ldk, ldv = _check_rows('page_write', k, 'k', T, Hk * D), _check_rows('page_write', v, 'v', T, Hk * D)
+    _check_here('page_write', k=k, v=v, k_cache=k_cache, v_cache=v_cache, slots=slots)
+    a = _lib.PageWriteArgs(k.data_ptr(), ldk, v.data_ptr(), ldv, k_cache.data_ptr(), v_cache.data_ptr(), s_page, s_head, s_row, slots.data_ptr(),
+                           T, Hk, D, page, n_pages, KV_TYPES[k_cache.dtype])
+    keep = (k, v, k_cache, v_cache, slots)
+    if _program is not None:
+        _program.append(('page_write', a, keep))
+        return
+    check(_lib.load().estts_page_write(a, _stream()), 'estts_page_write')
+    if _trace is not None or _debug_sync:
+        _record('page_write', {'T': T, 'H': Hk, 'depth': D, 'flops': 0.0, 'bytes': 2.0 * T * Hk * D * (4 + k_cache.element_size())},
+                _lib.load().estts_page_write, a, keep=keep)
+
+
+def paged_attention(q, k_cache, v_cache, block_table, lengths, ctx, heads, key_mask=None, scale=None, max_len=None):
+    """Attention of one new row per request over the rows in its pages (estts_paged_attention).  q, ctx: [B, >= heads * depth] float32
+    views; k_cache, v_cache: [n_pages, kv_heads, page, depth] (float32, bfloat16 or float16; any order of the first three dimensions in
+    memory), heads a multiple of kv_heads: query head h reads key head h // (heads / kv_heads); block_table [B, P], lengths [B] int32 as
+    page_plan leaves them (the new row is in its page already).  key_mask: [B, >= max_len] float32 view, rows with any value but 0 are
+    left out; a request with nothing left gets zeros.  scale: 1 / sqrt(depth) if None.  max_len: bound on the lengths that the host
+    knows of (P * page if None; rows past it are not read)."""
+    B = lengths.numel()
+    s_page, s_head, s_row = _check_pages('paged_attention', k_cache, v_cache)
+    _check_i32('paged_attention', lengths, 'lengths', (B,))
+    ld = _check_table('paged_attention', block_table, B)
+    n_pages, Hk, page, D = k_cache.shape
+    P = block_table.shape[1]
+    max_len = P * page if max_len is None else min(int(max_len), P * page)
+    if max_len < 1:
+        raise ValueError('paged_attention: max_len must be positive')
+    if heads < 1 or heads % Hk:
+        raise ValueError(f'paged_attention: {heads} query heads do not divide over {Hk} key heads')
+    width = heads * D
+    ldq, ldo = _check_rows('paged_attention', q, 'q', B, width), _check_rows('paged_attention', ctx, 'ctx', B, width)
+    sb = ss = 0
+    if key_mask is not None:
+        if key_mask.dtype != torch.float32:
+            raise TypeError(f'paged_attention: key_mask must be float32, got {key_mask.dtype}')
+        if key_mask.dim() != 2 or key_mask.shape[0] != B or key_mask.shape[1] < max_len:
+            raise ValueError(f'paged_attention: key_mask must be [{B}, >= {max_len}], got {list(key_mask.shape)}')
+        sb, ss = key_mask.stride()
+    _check_here('paged_attention', q=q, k_cache=k_cache, v_cache=v_cache, block_table=block_table, lengths=lengths, ctx=ctx, key_mask=key_mask)
+    lib, kind = _lib.load(), KV_TYPES[k_cache.dtype]
+    nbytes = lib.estts_paged_attention_ws_bytes(B, heads, Hk, D, kind, max_len)
+    ws = _scratch(nbytes, q.device) if nbytes > 0 else None
+    a = _lib.PagedAttentionArgs(q.data_ptr(), ldq, k_cache.data_ptr(), v_cache.data_ptr(), s_page, s_head, s_row,
+                                block_table.data_ptr(), ld, lengths.data_ptr(), _ptr(key_mask), sb, ss, ctx.data_ptr(),
+                                ldo, 1.0 / math.sqrt(D) if scale is None else scale, B, heads, Hk, D, page, n_pages, P,
+                                max_len, kind, _ptr(ws), max(nbytes, 0))
+    keep = (q, k_cache, v_cache, block_table, lengths, ctx, key_mask, ws)
+    if _program is not None:
+        _program.append(('paged_attention', a, keep))
+        return ctx
+    check(lib.estts_paged_attention(a, _stream()), 'estts_paged_attention')
+    if _trace is not None or _debug_sync:
+        _record('paged_attention', {'B': B, 'H': heads, 'kv_heads': Hk, 'depth': D, 'max_len': max_len, 'flops': 4.0 * B * heads * max_len * D,
+                                    'bytes': 2.0 * B * max_len * Hk * D * k_cache.element_size()},
+                lib.estts_paged_attention, a, keep=keep)
+    return ctx
 
 
 def rownorm_args(y, out, ln_a=None, act=None, residual=None, ln_b=None, eps=1e-6, M=None, D=None,

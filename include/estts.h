@@ -29,7 +29,7 @@
 extern "C" {
 #endif
 
-#define ESTTS_ABI_VERSION 36
+#define ESTTS_ABI_VERSION 37
 
 /* activation codes for estts_gemm / estts_rownorm */
 #define ESTTS_ACT_NONE 0
@@ -882,6 +882,87 @@ typedef struct estts_prenet_row_args {
 int estts_prenet_row(const estts_prenet_row_args* args, void* stream);
 
 /* ------------------------------------------------------------------------------------------
+ * Paged key / value memory: several utterances decode side by side out of one cache that is cut into pages of `page` rows, so
+ * that a request holds what its length needs and no more.  No counterpart in the reference, whose decoder loop runs one
+ * utterance at a time and keeps no cache (model/AutoregressiveTransformer.py:265-296).
+ *
+ *   k_cache, v_cache [n_pages, heads, page, depth]   elements of type ESTTS_KV_*; strides s_page, s_head, s_row in elements (equal for
+ *                                                    both, so either order of heads and rows will do), depth contiguous
+ *   block_table      [B, P]  int32, row stride ld_table: page j of request b holds its rows [j page, (j + 1) page)
+ *   lengths          [B]     int32: rows request b has in its pages
+ *   slot             page id * page + row inside the page; -1 = no place
+ * page is a multiple of 16.  Ids outside [0, n_pages), slots outside [0, n_pages page) and lengths outside [0, P page] reach no memory:
+ * such rows are neither written nor read, and such lengths count as the nearest bound.
+ * ------------------------------------------------------------------------------------------ */
+#define ESTTS_KV_F32 0
+#define ESTTS_KV_BF16 1
+#define ESTTS_KV_F16 2
+
+/* The page plan of a step: n_new[b] >= 0 rows are about to come for request b; n_new[b] < 0 says that the request has ended.
+ * free_pages [n_pages] is a stack of unused page ids with n_free[0] entries.
+ *   used_b = ceil(lengths[b] / page)
+ *   1. the pages of the requests that ended go onto the stack, in the order of b and of their pages
+ *   2. a request whose rows fit (its table row is long enough, its rows, if any, lie inside the slot map) needs
+ *      need_b = ceil((lengths[b] + n_new[b]) / page) - used_b more pages and is granted iff need_b = 0 or the sum of need over the
+ *      requests up to and including b is at most the height of the stack; the granted ones take their pages off the top in the
+ *      order of b: block_table[b, used_b + i], i < need_b
+ *   3. row i of request b goes to slots[r], positions[r] = lengths[b] + i (positions may be NULL), r = i + sum of n_new over the
+ *      requests before b (R = 0: packed, T rows in the map) or r = b R + i (R > 0: padded, T = B R); all other entries of the two maps,
+ *      those of refused requests among them, become -1
+ *   lengths_out[b] = 0 (ended), lengths[b] + n_new[b] (granted) or lengths[b] (refused);  n_free_out[0] = height of the stack now;
+ *   refused[0] = number of requests that asked and were not granted (may be NULL)
+ * lengths_out may be lengths and n_free_out may be n_free (the state of a decoding loop); block_table and free_pages are updated in
+ * place, and only where the rules above write.  ws: 3 B int32 of scratch that belong to this call until it has run. */
+typedef struct estts_page_plan_args {
+    const int32_t* lengths; const int32_t* n_new;
+    int32_t* block_table; int64_t ld_table;
+    int32_t* free_pages; const int32_t* n_free;
+    int32_t* slots; int32_t* positions;
+    int32_t* lengths_out; int32_t* n_free_out; int32_t* refused;
+    int32_t* ws;
+    int32_t B, P, n_pages, page, T, R;
+} estts_page_plan_args;
+
+int estts_page_plan(const estts_page_plan_args* args, void* stream);
+
+/* K / V rows into the pages: for t < T with 0 <= slots[t] < n_pages page, rows k[t], v[t] (float32, head h at columns [h depth, (h + 1) depth))
+ * go to that slot, rounded to the cache's type (to nearest, ties to even); everything else stays as it was.  The slots of one call
+ * are distinct (estts_page_plan's are): where two rows name the same slot, which of the two it holds afterwards is not defined. */
+typedef struct estts_page_write_args {
+    const float* k; int64_t ldk;
+    const float* v; int64_t ldv;
+    void* k_cache; void* v_cache; int64_t s_page, s_head, s_row;
+    const int32_t* slots;
+    int32_t T, heads, depth, page, n_pages, type;
+} estts_page_write_args;
+
+int estts_page_write(const estts_page_write_args* args, void* stream);
+
+/* Attention of one new row per request over the request's pages:
+ *   s_j = scale q[b, h] . k_j   for the rows j < min(lengths[b], max_len) with key_mask[b, j] == 0
+ *   ctx[b, h] = sum_j softmax(s)_j v_j;   a request without such rows gets zeros
+ * q [B, H depth] and ctx [B, H depth] float32 (row strides ldq, ldo), H a multiple of kv_heads: query head h reads key head
+ * h / (H / kv_heads).  depth 32, 64 or 128.  key_mask (may be NULL) float32 with strides mask_sb (request) and mask_ss (position): any value
+ * but 0 leaves the row out, whatever the row holds (estts_attention adds -1e9 instead, so that a fully masked row there is a
+ * mean of the values).  max_len bounds the lengths (0: P page); it decides how the work is split, and a low bound lets short
+ * requests run in one launch.  Products and sums have float32 accuracy for every cache type.
+ * ws: estts_paged_attention_ws_bytes() bytes (may be NULL where that is 0) that belong to this call until it has run. */
+typedef struct estts_paged_attention_args {
+    const float* q; int64_t ldq;
+    const void* k_cache; const void* v_cache; int64_t s_page, s_head, s_row;
+    const int32_t* block_table; int64_t ld_table;
+    const int32_t* lengths;
+    const float* key_mask; int64_t mask_sb, mask_ss;
+    float* ctx; int64_t ldo;
+    float scale;
+    int32_t B, H, kv_heads, depth, page, n_pages, P, max_len, type;
+    void* ws; int64_t ws_bytes;
+} estts_paged_attention_args;
+
+int estts_paged_attention(const estts_paged_attention_args* args, void* stream);
+int64_t estts_paged_attention_ws_bytes(int32_t B, int32_t H, int32_t kv_heads, int32_t depth, int32_t type, int32_t max_len);
+
+/* ------------------------------------------------------------------------------------------
  * Step programs: a fixed sequence of launches whose arguments depend affinely on a step index (an incremental decoder:
  * row i of a cache, a key range of i + 1, ...).  Each op carries the argument block of step 0 and a patch list; at step s
  * the field at byte `offset` of a copy of the block is advanced by s * stride (a pointer, in bytes, or an int32), then the
@@ -889,7 +970,8 @@ int estts_prenet_row(const estts_prenet_row_args* args, void* stream);
  * in the host language.  No counterpart in the reference (its loop, model/AutoregressiveTransformer.py:279-296, re-runs
  * the whole Keras decoder every step).
  * kind: 0 estts_gemm, 1 estts_attention, 2 estts_rownorm, 3 estts_row_zero_mask (args = estts_rowmask_args),
- * 4 estts_cross_attention_row, 5 estts_decoder_block_row, 6 estts_prenet_row.
+ * 4 estts_cross_attention_row, 5 estts_decoder_block_row, 6 estts_prenet_row, 7 estts_page_plan, 8 estts_page_write,
+ * 9 estts_paged_attention.
  * ------------------------------------------------------------------------------------------ */
 typedef struct estts_rowmask_args {
     const float* x; int32_t ldx;

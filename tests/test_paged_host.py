@@ -1,0 +1,148 @@
+"""Paged decoding without a GPU: what the entry points refuse (the C ABI with pointers that are never followed, the Python layer with
+CPU tensors), the layout of the argument blocks, and models of the kernels' index arithmetic with bad pages, slots and lengths."""
+import ctypes
+import os
+import subprocess
+
+import pytest
+import torch
+
+import estts
+from estts import _lib, ops
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+FAKE = 0x1000
+BLOCKS = {'estts_page_plan_args': _lib.PagePlanArgs, 'estts_page_write_args': _lib.PageWriteArgs,
+          'estts_paged_attention_args': _lib.PagedAttentionArgs}
+
+
+@pytest.mark.parametrize('cname', sorted(BLOCKS))
+def test_field_offsets_match_header_layout(tmp_path, cname):
+    cls = BLOCKS[cname]
+    names = [n for n, _ in cls._fields_]
+    src = tmp_path / 'offsets.c'
+    src.write_text('#include <stdio.h>\n#include <stddef.h>\n#include "estts.h"\nint main(void) {\n' +
+                   ''.join(f'  printf("{n} %zu\\n", offsetof({cname}, {n}));\n' for n in names) +
+                   f'  printf("sizeof %zu\\n", sizeof({cname}));\n  return 0;\n}}\n')
+    exe = tmp_path / 'offsets'
+    subprocess.run(['gcc', '-I', os.path.join(ROOT, 'include'), str(src), '-o', str(exe)], check=True)
+    at = dict(line.split() for line in subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.strip().splitlines())
+    assert ctypes.sizeof(cls) == int(at['sizeof'])
+    for n in names:
+        assert getattr(cls, n).offset == int(at[n]), n
+
+
+# ---------------------------------------------------------------------------------------------------------------- C ABI refusals
+def plan_block(**kw):
+    f = dict(lengths=FAKE, n_new=FAKE, block_table=FAKE, ld_table=8, free_pages=FAKE, n_free=FAKE, slots=FAKE, positions=FAKE, lengths_out=FAKE,
+             n_free_out=FAKE, refused=FAKE, ws=FAKE, B=4, P=8, n_pages=32, page=16, T=4, R=1)
+    f.update(kw)
+    return _lib.PagePlanArgs(**f)
+
+
+def write_block(**kw):
+    f = dict(k=FAKE, ldk=256, v=FAKE, ldv=256, k_cache=FAKE, v_cache=FAKE, s_page=4096, s_head=1024, s_row=64, slots=FAKE, T=4, heads=4, depth=64,
+             page=16, n_pages=32, type=0)
+    f.update(kw)
+    return _lib.PageWriteArgs(**f)
+
+
+def attention_block(**kw):
+    f = dict(q=FAKE, ldq=256, k_cache=FAKE, v_cache=FAKE, s_page=4096, s_head=1024, s_row=64, block_table=FAKE, ld_table=8, lengths=FAKE, ctx=FAKE,
+             ldo=256, scale=0.125, B=4, H=4, kv_heads=4, depth=64, page=16, n_pages=32, P=8, max_len=128, type=0)
+    f.update(kw)
+    return _lib.PagedAttentionArgs(**f)
+
+
+@pytest.mark.parametrize('bad,word', [(dict(lengths=None), 'null'), (dict(ws=None), 'null'), (dict(B=0), 'shape'), (dict(T=0), 'shape'),
+                                      (dict(ld_table=7), 'shape'), (dict(R=2), 'padded'), (dict(page=8), 'multiple of 16'), (dict(page=0), 'multiple of 16'),
+                                      (dict(page=24), 'multiple of 16'), (dict(n_pages=1 << 27), '2^31'), (dict(P=1 << 27, ld_table=1 << 27), '2^31')])
+def test_page_plan_refuses(bad, word):
+    lib = _lib.load()
+    assert lib.estts_page_plan(plan_block(**bad), None) != 0
+    assert word in lib.estts_last_error().decode(), lib.estts_last_error()
+
+
+@pytest.mark.parametrize('bad,word', [(dict(k=None), 'null'), (dict(slots=None), 'null'), (dict(T=0), 'shape'), (dict(depth=60), 'depth'),
+                                      (dict(depth=4096), 'depth'), (dict(page=20), 'multiple of 16'), (dict(type=3), 'type'), (dict(ldk=128), 'rows'),
+                                      (dict(ldv=258), 'rows'), (dict(k=FAKE + 4), 'rows'), (dict(k_cache=FAKE + 8), '16 bytes'),
+                                      (dict(s_head=1022), '16 bytes'), (dict(type=1, s_page=4100), '16 bytes'), (dict(s_row=32), '16 bytes'),
+                                      (dict(n_pages=1 << 27), '2^31')])
+def test_page_write_refuses(bad, word):
+    lib = _lib.load()
+    assert lib.estts_page_write(write_block(**bad), None) != 0
+    assert word in lib.estts_last_error().decode(), lib.estts_last_error()
+
+
+@pytest.mark.parametrize('bad,word', [(dict(q=None), 'null'), (dict(lengths=None), 'null'), (dict(B=0), 'shape'), (dict(B=65536), 'shape'),
+                                      (dict(H=6), 'shape'), (dict(depth=48), 'depth'), (dict(depth=256), 'depth'), (dict(page=12), 'multiple of 16'),
+                                      (dict(type=-1), 'type'), (dict(ldq=192), 'query rows'), (dict(ldo=255), 'query rows'),
+                                      (dict(q=FAKE + 8), 'query rows'), (dict(s_row=66), '16 bytes'), (dict(k_cache=FAKE + 2), '16 bytes'),
+                                      (dict(max_len=-1), 'max_len'), (dict(s_row=1 << 25), '2^28'), (dict(n_pages=1 << 27), '2^31')])
+def test_paged_attention_refuses(bad, word):
+    lib = _lib.load()
+    assert lib.estts_paged_attention(attention_block(**bad), None) != 0
+    assert word in lib.estts_last_error().decode(), lib.estts_last_error()
+
+
+def test_null_blocks_are_refused():
+    lib = _lib.load()
+    for name in ('estts_page_plan', 'estts_page_write', 'estts_paged_attention'):
+        assert getattr(lib, name)(None, None) != 0 and b'null args' in lib.estts_last_error()
+
+
+# ------------------------------------------------------------------------------------------------------------- Python refusals
+def i32(*shape):
+    return torch.zeros(*shape, dtype=torch.int32)
+
+
+def plan_call(**kw):
+    f = dict(lengths=i32(4), new=i32(4), block_table=i32(4, 8), free_pages=i32(32), n_free=i32(1), page=16, slots=i32(4, 1))
+    f.update(kw)
+    return ops.page_plan(**f)
+
+
+@pytest.mark.parametrize('bad,error', [(dict(), 'is on cpu'), (dict(new=i32(3)), 'new'), (dict(new=torch.zeros(4)), 'int32'), (dict(block_table=i32(3, 8)), 'block_table'),
+                                       (dict(block_table=i32(8, 4).t()), 'block_table'), (dict(block_table=i32(4, 8).long()), 'int32'), (dict(slots=i32(3, 1)), 'slots'),
+                                       (dict(slots=i32(2, 2, 1)), 'slots'), (dict(slots=i32(4, 2)[:, :1]), 'slots'), (dict(positions=i32(4)), 'positions'),
+                                       (dict(lengths_out=i32(5)), 'lengths_out'), (dict(n_free=i32(2)), 'n_free'), (dict(refused=i32(4)), 'refused')])
+def test_page_plan_checks_its_arguments(bad, error):
+    with pytest.raises((ValueError, TypeError), match=error):
+        plan_call(**bad)
+
+
+def caches(**kw):
+    return torch.zeros(32, 4, 16, 64, **kw), torch.zeros(32, 4, 16, 64, **kw)
+
+
+@pytest.mark.parametrize('bad,error', [(dict(), 'is on cpu'), (dict(k=torch.zeros(4, 128)), 'k must be'), (dict(v=torch.zeros(5, 256)), 'v must be'),
+                                       (dict(k=torch.zeros(256, 4).t()), 'k must be'), (dict(k=torch.zeros(4, 256).bfloat16()), 'float32'), (dict(slots=torch.zeros(4)), 'int32'),
+                                       (dict(k_cache=torch.zeros(32, 4, 16, 64).double(), v_cache=torch.zeros(32, 4, 16, 64).double()), 'float16'),
+                                       (dict(k_cache=torch.zeros(32, 4, 16, 64).half()), 'same strides'), (dict(k_cache=torch.zeros(32, 16, 4, 64).transpose(1, 2)), 'same strides'),
+                                       (dict(k_cache=torch.zeros(1, 4, 16, 64).expand(32, 4, 16, 64), v_cache=torch.zeros(1, 4, 16, 64).expand(32, 4, 16, 64)), 'broadcast'),
+                                       (dict(k_cache=torch.zeros(32, 4, 64, 16).transpose(2, 3), v_cache=torch.zeros(32, 4, 64, 16).transpose(2, 3)), 'contiguous')])
+def test_page_write_checks_its_arguments(bad, error):
+    k_cache, v_cache = caches()
+    f = dict(k=torch.zeros(4, 256), v=torch.zeros(4, 256), k_cache=k_cache, v_cache=v_cache, slots=i32(4))
+    f.update(bad)
+    with pytest.raises((ValueError, TypeError), match=error):
+        ops.page_write(**f)
+
+
+@pytest.mark.parametrize('bad,error', [(dict(), 'is on cpu'), (dict(q=torch.zeros(4, 255)), 'q must be'), (dict(ctx=torch.zeros(3, 256)), 'ctx must be'),
+                                       (dict(q=torch.zeros(4, 256).half()), 'float32'), (dict(heads=6), 'do not divide'), (dict(heads=0), 'do not divide'),
+                                       (dict(lengths=i32(4).long()), 'int32'), (dict(block_table=i32(5, 8)), 'block_table'), (dict(max_len=0), 'max_len'),
+                                       (dict(key_mask=torch.zeros(4, 127)), 'key_mask'), (dict(key_mask=torch.zeros(4, 128, dtype=torch.bool)), 'key_mask'),
+                                       (dict(key_mask=torch.zeros(3, 128)), 'key_mask')])
+def test_paged_attention_checks_its_arguments(bad, error):
+    k_cache, v_cache = caches()
+    f = dict(q=torch.zeros(4, 256), k_cache=k_cache, v_cache=v_cache, block_table=i32(4, 8), lengths=i32(4), ctx=torch.zeros(4, 256), heads=4)
+    f.update(bad)
+    with pytest.raises((ValueError, TypeError), match=error):
+        ops.paged_attention(**f)
+
+
+def test_pages_must_be_a_multiple_of_sixteen_rows():
+    lib = _lib.load()
+    for page in (1, 8, 15, 17, 40):
+        assert lib.estts_page_plan(plan_block(page=page), None) != 0 and b'multiple of 16' in lib.estts_last_error()
