@@ -120,7 +120,7 @@ class PrenetRowArgs(C.Structure):
 
 class PagePlanArgs(C.Structure):
     _fields_ = [('lengths', _vp), ('n_new', _vp), ('block_table', _vp), ('ld_table', _i64), ('free_pages', _vp), ('n_free', _vp),
-                ('slots', _vp), ('positions', _vp), ('lengths_out', _vp), ('n_free_out', _vp), ('refused', _vp), ('ws', _vp),
+                ('slots', _vp), ('positions', _vp), ('lengths_out', _vp), ('n_free_out', _vp), ('refused', _vp), ('ws', _vp), ('ws_bytes', _i64),
                 ('B', _i32), ('P', _i32), ('n_pages', _i32), ('page', _i32), ('T', _i32), ('R', _i32)]
 
 
@@ -216,9 +216,10 @@ SIGNATURES = {
     'estts_decoder_block_row': (_i32, [C.POINTER(DecoderBlockArgs), _vp]),
     'estts_prenet_row': (_i32, [C.POINTER(PrenetRowArgs), _vp]),
     'estts_page_plan': (_i32, [C.POINTER(PagePlanArgs), _vp]),
+    'estts_page_plan_ws_bytes': (_i64, [_i32, _i32]),
     'estts_page_write': (_i32, [C.POINTER(PageWriteArgs), _vp]),
     'estts_paged_attention': (_i32, [C.POINTER(PagedAttentionArgs), _vp]),
-    'estts_paged_attention_ws_bytes': (_i64, [_i32, _i32, _i32, _i32, _i32, _i32]),
+    'estts_paged_attention_ws_bytes': (_i64, [_i32, _i32, _i32, _i32, _i32]),
     'estts_masked_mae': (_i32, [_vp, _i32, _vp, _i32, _vp, _i32, _i32, _vp]),
     'estts_wavernn_prep': (_i32, [C.POINTER(WavernnPrepArgs), _vp]),
     'estts_gru_gates': (_i32, [_vp, _i32, _vp, _i32, _vp, _i32, _vp, _i32, _vp, _i32, _i32, _i32, _vp]),

@@ -7,12 +7,15 @@
 namespace {
 
 // ------------------------------------------------------------------------------------------------ page plan
-constexpr int PLAN_THREADS = 1024;
+// Whole-number work on a few kilobytes, bound by latency: a launch, the lengths, the scans, the stack or the table, the maps.  One
+// workgroup scans the requests; the copies and the rows' places are then made by the same workgroup, or by a second launch
+// of as many as it takes where there are more of them than PLAN_ROWS.
+constexpr int PLAN_LDS = 4096;         // requests whose plan fits the LDS (four ints each); beyond that it lives in the caller's scratch
 
 __device__ __forceinline__ int pages_of(int rows, int page) { return (int)(((unsigned)rows + page - 1) / (unsigned)page); }
 
-// inclusive prefix sum over the workgroup's threads, and the total
-template <typename V>
+// inclusive prefix sum over the workgroup's NT threads, and the total
+template <int NT, typename V>
 __device__ __forceinline__ V block_scan(V v, V* part, V& total) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
@@ -26,7 +29,7 @@ __device__ __forceinline__ V block_scan(V v, V* part, V& total) {
     V before = 0;
     total = 0;
 #pragma unroll
-    for (int w = 0; w < PLAN_THREADS / 64; ++w) {
+    for (int w = 0; w < NT / 64; ++w) {
         const V s = part[w];
         if (w < wave) before += s;
         total += s;
@@ -44,93 +47,136 @@ __device__ __forceinline__ int first_past(const int* end, int B, int x) {
     return lo;
 }
 
-// One workgroup.  ws holds per request: end of its rows in a packed slot map (at most T), pages granted up to and including it, and its
-// length (complemented where it gets no rows).
-__global__ __launch_bounds__(PLAN_THREADS) void page_plan_kernel(const estts_page_plan_args p) {
-    __shared__ int part_i[16];
-    __shared__ long long part_l[16];
-    const int tid = threadIdx.x;
-    const int cap = p.P * p.page;
-    int* const row_end = p.ws;
-    int* const page_end = p.ws + p.B;
-    int* const len_of = p.ws + 2 * (long)p.B;
+// What is known of each request after the scans.  Up to PLAN_LDS requests it is held in the LDS.
+struct PagePlan {
+    const int* row_end;        // end of its rows in a packed map (at most T)
+    const int* back_end;       // pages given back up to and including it
+    const int* page_end;       // pages granted up to and including it
+    const int* len_of;         // its length, complemented where it gets no rows
+    int height0, back, taken;  // the stack before the call, pages that come back to it, pages that are then taken off it
+};
+constexpr int PLAN_HEAD = 4;   // scratch of a plan in two launches: height0, back, taken, then the four arrays
 
-    const int height0 = min(max(p.n_free[0], 0), p.n_pages);
-    // 1. pages of the requests that ended
-    int back = 0;
-    for (int b0 = 0; b0 < p.B; b0 += PLAN_THREADS) {
-        const int b = b0 + tid;
-        const bool ended = b < p.B && p.n_new[b] < 0;
-        const int used = ended ? pages_of(min(max(p.lengths[b], 0), cap), p.page) : 0;
-        int total;
-        const int upto = block_scan(used, part_i, total);
-        if (b < p.B) page_end[b] = back + upto;
-        back += total;
-    }
-    __syncthreads();
-    back = min(back, p.n_pages - height0);          // (more would be pages that are held twice)
-    for (int g = tid; g < back; g += PLAN_THREADS) {
-        const int b = first_past(page_end, p.B, g);
-        const int j = g - (b ? page_end[b - 1] : 0);
-        p.free_pages[height0 + g] = p.block_table[b * p.ld_table + j];
-    }
-    const int height = height0 + back;
-    __syncthreads();
-    // 2. grants
-    int asked = 0, taken = 0, refused = 0;
-    long long rows = 0;
-    for (int b0 = 0; b0 < p.B; b0 += PLAN_THREADS) {
-        const int b = b0 + tid;
-        const int n = b < p.B ? p.n_new[b] : 0;
-        const int len = b < p.B ? min(max(p.lengths[b], 0), cap) : 0;
-        const long long want = max(n, 0);
-        long long rows_total;
-        const long long rows_upto = rows + block_scan(want, part_l, rows_total);
-        const bool fits = b < p.B && n >= 0 && len + want <= cap && (want == 0 || (p.R ? want <= p.R : rows_upto <= p.T));
-        const int need = fits ? pages_of(len + (int)want, p.page) - pages_of(len, p.page) : 0;
-        int need_total;
-        const int upto = asked + block_scan(need, part_i, need_total);
-        const bool granted = fits && (need == 0 || upto <= height);
-        int refused_total, taken_total;
-        block_scan((int)(b < p.B && n >= 0 && !granted), part_i, refused_total);
-        block_scan(granted ? need : 0, part_i, taken_total);
-        if (b < p.B) {
-            row_end[b] = (int)min(rows_upto, (long long)p.T);
-            page_end[b] = min(upto, height);        // (a request that is turned away ends no page below its own)
-            len_of[b] = granted ? len : ~len;
-            p.lengths_out[b] = n < 0 ? 0 : granted ? len + (int)want : len;
-        }
-        rows += rows_total;
-        asked += need_total;
-        taken += taken_total;
-        refused += refused_total;
-    }
-    __syncthreads();
-    for (int g = tid; g < taken; g += PLAN_THREADS) {
-        const int b = first_past(page_end, p.B, g);
-        const int i = g - (b ? page_end[b - 1] : 0);
-        p.block_table[b * p.ld_table + pages_of(len_of[b], p.page) + i] = p.free_pages[height - 1 - g];
-    }
-    if (tid == 0) {
-        p.n_free_out[0] = height - taken;
-        if (p.refused) p.refused[0] = refused;
-    }
-    __syncthreads();
-    // 3. where each row goes
-    for (int t = tid; t < p.T; t += PLAN_THREADS) {
-        const int b = p.R ? t / p.R : first_past(row_end, p.B, t);
+// The copies that a plan asks for, in any order and by any thread: every source is as the call found it.  Place e of the stack with the
+// given-back pages on it is free_pages[e] below height0, above it the page of an ended request; a row's page is in the table if the
+// request held it already, else on the stack.
+__device__ __forceinline__ void carry_out(const estts_page_plan_args& p, const PagePlan& q, const int first, const int step) {
+    auto given_back = [&](int g) {
+        const int b = first_past(q.back_end, p.B, g);
+        return p.block_table[b * p.ld_table + (g - (b ? q.back_end[b - 1] : 0))];
+    };
+    auto on_stack = [&](int e) { return e < q.height0 ? p.free_pages[e] : given_back(e - q.height0); };
+    const int height = q.height0 + q.back;
+    for (int t = first; t < p.T; t += step) {
+        const int b = p.R ? t / p.R : first_past(q.row_end, p.B, t);
         int slot = -1, pos = -1;
-        if (b < p.B && len_of[b] >= 0) {
-            const int i = p.R ? t - b * p.R : t - (b ? row_end[b - 1] : 0);
+        const int len = b < p.B ? q.len_of[b] : -1;
+        if (len >= 0) {
+            const int i = p.R ? t - b * p.R : t - (b ? q.row_end[b - 1] : 0);
             if (!p.R || i < p.n_new[b]) {
-                pos = len_of[b] + i;
-                const int id = p.block_table[b * p.ld_table + pos / p.page];
-                if (id >= 0 && id < p.n_pages) slot = id * p.page + pos % p.page;
+                pos = len + i;
+                const int j = pos / p.page, fresh = j - pages_of(len, p.page);
+                const int id = fresh < 0 ? p.block_table[b * p.ld_table + j] : on_stack(height - 1 - ((b ? q.page_end[b - 1] : 0) + fresh));
+                if (id >= 0 && id < p.n_pages) slot = id * p.page + (pos - j * p.page);
             }
         }
         p.slots[t] = slot;
         if (p.positions) p.positions[t] = pos;
     }
+    for (int g = first; g < q.taken; g += step) {
+        const int b = first_past(q.page_end, p.B, g);
+        const int i = g - (b ? q.page_end[b - 1] : 0);
+        p.block_table[b * p.ld_table + pages_of(q.len_of[b], p.page) + i] = on_stack(height - 1 - g);
+    }
+#pragma unroll 4
+    for (int g = first; g < q.back; g += step) p.free_pages[q.height0 + g] = given_back(g);
+}
+
+// The scans, by one workgroup; then the copies, unless they are left to page_copy_kernel (split != 0; the plan goes to p.ws).
+template <int NT, bool LDS>
+__global__ __launch_bounds__(NT) void page_plan_kernel(const estts_page_plan_args p, const int split) {
+    __shared__ int part_i[NT / 64];
+    __shared__ long long part_l[NT / 64];
+    __shared__ int taken_s, refused_s;
+    __shared__ int plan_s[LDS ? 4 * PLAN_LDS : 1];
+    const int tid = threadIdx.x;
+    const int cap = p.P * p.page;
+    const long pitch = LDS ? PLAN_LDS : p.B;
+    int* const plan = LDS ? plan_s : p.ws + PLAN_HEAD;
+    int *const row_end = plan, *const back_end = plan + pitch, *const page_end = plan + 2 * pitch, *const len_of = plan + 3 * pitch;
+
+    const int height0 = min(max(p.n_free[0], 0), p.n_pages);
+    if (tid == 0) taken_s = refused_s = 0;
+    // rows before each request; pages of the requests that ended
+    int back = 0;
+    long long rows_before = 0;
+    for (int b0 = 0; b0 < p.B; b0 += NT) {
+        const int b = b0 + tid;
+        const int n = b < p.B ? p.n_new[b] : 0;
+        const int len = b < p.B ? min(max(p.lengths[b], 0), cap) : 0;
+        int back_total;
+        const int upto = back + block_scan<NT>(n < 0 ? pages_of(len, p.page) : 0, part_i, back_total);
+        long long rows_total;
+        const long long rows_upto = rows_before + block_scan<NT>((long long)max(n, 0), part_l, rows_total);
+        if (b < p.B) {
+            back_end[b] = upto;
+            const bool inside = n <= 0 || (p.R ? n <= p.R : rows_upto <= p.T);
+            row_end[b] = (int)min(rows_upto, (long long)p.T);
+            len_of[b] = inside ? len : ~len;
+        }
+        back += back_total;
+        rows_before += rows_total;
+    }
+    back = min(back, p.n_pages - height0);          // (more would be pages that are held twice)
+    const int height = height0 + back;
+    // grants
+    int asked = 0;
+    for (int b0 = 0; b0 < p.B; b0 += NT) {
+        const int b = b0 + tid;
+        const int n = b < p.B ? p.n_new[b] : 0;
+        const int mark = b < p.B ? len_of[b] : 0, len = mark < 0 ? ~mark : mark;
+        const bool fits = b < p.B && n >= 0 && mark >= 0 && len + (long long)n <= cap;
+        const int need = fits ? pages_of(len + n, p.page) - pages_of(len, p.page) : 0;
+        int need_total;
+        const int upto = asked + block_scan<NT>(need, part_i, need_total);
+        const bool granted = fits && (need == 0 || upto <= height);
+        if (b < p.B) {
+            page_end[b] = min(upto, height);        // (a request that is turned away ends no page below its own)
+            len_of[b] = granted ? len : ~len;
+            p.lengths_out[b] = n < 0 ? 0 : granted ? len + n : len;
+            if (granted && need) atomicMax(&taken_s, upto);
+            if (n >= 0 && !granted) atomicAdd(&refused_s, 1);
+        }
+        asked += need_total;
+    }
+    __syncthreads();
+    const int taken = taken_s;
+    if (tid == 0) {
+        p.n_free_out[0] = height - taken;
+        if (p.refused) p.refused[0] = refused_s;
+    }
+    if (split) {
+        if (tid == 0) { p.ws[0] = height0; p.ws[1] = back; p.ws[2] = taken; }
+        if (LDS)
+            for (int b = tid; b < p.B; b += NT)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) p.ws[PLAN_HEAD + k * p.B + b] = plan[k * pitch + b];
+        return;
+    }
+    carry_out(p, {row_end, back_end, page_end, len_of, height0, back, taken}, tid, NT);
+}
+
+template <bool LDS>
+__global__ __launch_bounds__(256) void page_copy_kernel(const estts_page_plan_args p) {
+    __shared__ int plan_s[LDS ? 4 * PLAN_LDS : 1];
+    const int* plan = p.ws + PLAN_HEAD;
+    const int height0 = p.ws[0], back = p.ws[1], taken = p.ws[2];
+    if (LDS) {
+        for (int x = threadIdx.x; x < 4 * p.B; x += 256) plan_s[x] = plan[x];
+        __syncthreads();
+        plan = plan_s;
+    }
+    carry_out(p, {plan, plan + p.B, plan + 2 * (long)p.B, plan + 3 * (long)p.B, height0, back, taken}, blockIdx.x * 256 + threadIdx.x, gridDim.x * 256);
 }
 
 // ------------------------------------------------------------------------------------------------ rows into the pages
@@ -172,9 +218,12 @@ __global__ __launch_bounds__(256) void page_write_kernel(const estts_page_write_
 // Scores, maxima, sums and outputs are float32.
 
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
-typedef __attribute__((ext_vector_type(2))) _Float16 f16x2_t;
 
-constexpr int ATT_WAVES = 4;
+constexpr int ATT_WAVES = 4;           // waves of a workgroup (8 and 16 gain nothing: a wave's arithmetic fills its SIMD's share)
+constexpr int FEW_QUERIES = 2;         // query heads per key head up to which float32 pages take the vector ALU
+
+// 16-row halves of a wave's tile
+constexpr int tile_halves(int depth, int esize) { return depth * esize == 512 ? 1 : 2; }
 
 template <typename T> struct Kv16 { typedef bf16x8 Frag; static constexpr int PIECES = 1; };      // (float32: not used)
 template <> struct Kv16<__bf16> {
@@ -204,466 +253,717 @@ __device__ __forceinline__ void split_pieces(const float (&x)[8], typename Kv16<
         }
 }
 
-// The share of the work that workgroup `item` of a key head does: rows [begin, end) of request b, split `split` of `n_split`
-struct PagedWork { int b, begin, end, split, n_split, first; bool any; };
-
 __device__ __forceinline__ int request_rows(const estts_paged_attention_args& p, int b) {
     return min(min(max(p.lengths[b], 0), p.P * p.page), p.max_len);
 }
 
-__device__ __forceinline__ int wave_sum_int(int v) {
-#pragma unroll
-    for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
-    return v;
-}
+// How the rows are dealt out.  target == 0: a workgroup has a whole request (and a key head's queries).  Else all rows of all requests,
+// in units of UNIT, are one line that is cut into equal parts, so that long and short requests keep the chip equally busy and no part
+// is last; the host knows no lengths, the parts follow from them on the GPU.  A part holds whole requests, the end of one that began in
+// an earlier part and the beginning of one that goes on in a later part: two places of scratch a part, 2k and 2k + 1, hold the latter two.
+struct PagedSegment { int b, begin, end, place; bool whole; };      // rows [begin, end) of request b; place: of the scratch, unless whole
 
-// Rows are dealt out in chunks of equal size over all requests, so that long and short requests keep the chip equally busy: about
-// `target` chunks, each request at least one, so at most target + B items (the grid).  Every wave finds its own from the lengths.
-__device__ __forceinline__ PagedWork find_work(const estts_paged_attention_args& p, int item, int target, int min_rows) {
-    PagedWork w;
-    if (target == 0) {
-        w.b = item; w.begin = 0; w.end = request_rows(p, item); w.split = 0; w.n_split = 1; w.first = item; w.any = true;
-        return w;
-    }
-    const int lane = threadIdx.x & 63;
-    constexpr int UNIT = 32 * ATT_WAVES;            // one round of the workgroup's waves over tiles of 32 rows
-    int units = 0;                                  // (at most 2^31 / 128 a request: the caller keeps B * P * page / 128 below 2^31)
-    for (int b = lane; b < p.B; b += 64) units += (request_rows(p, b) + UNIT - 1) / UNIT;
-    units = wave_sum_int(units);
-    const int chunk = max((units + target - 1) / target, min_rows / UNIT) * UNIT;
-    w.any = false;
-    int before = 0;
-    for (int b0 = 0; b0 < p.B; b0 += 64) {
-        const int rows = b0 + lane < p.B ? request_rows(p, b0 + lane) : 0;
-        const int n = b0 + lane < p.B ? max((rows - 1) / chunk + 1, 1) : 0;
-        int upto = n;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const int up = __shfl_up(upto, d);
-            if (lane >= d) upto += up;
-        }
-        const uint64_t past = __ballot(before + upto > item);
-        if (past) {
-            const int l = __ffsll((unsigned long long)past) - 1;
-            w.b = b0 + l;
-            w.n_split = __shfl(n, l);
-            w.first = before + __shfl(upto, l) - w.n_split;
-            w.split = item - w.first;
-            const int len = __shfl(rows, l);
-            w.begin = w.split * chunk;
-            w.end = min(len, w.begin + chunk);
-            w.any = true;
-            break;
-        }
-        before += __shfl(upto, 63);
-    }
-    return w;
-}
+template <int NT, int UNIT>
+struct PagedPart {
+    int k, parts, b, off, left, total, at;      // requests from b on, of b the units from off on, left units in all; at: place of unit off of b in the line
 
-// scratch of a split call: per item and query head the unnormalised output (relative to its maximum), then (maximum, sum); per request
-// (first item, number of items)
-struct PagedScratch {
-    float* out; float2* ml; int2* items;
-    __host__ __device__ PagedScratch(void* ws, long n_items, int H, int depth) {
-        out = static_cast<float*>(ws);
-        ml = reinterpret_cast<float2*>(out + n_items * H * depth);
-        items = reinterpret_cast<int2*>(ml + n_items * H);
+    static __device__ __forceinline__ int units_of(int rows) { return max((rows + UNIT - 1) / UNIT, 1); }      // (a request without rows still gets its zeros)
+
+    __device__ __forceinline__ bool find(const estts_paged_attention_args& p, int part, int target) {
+        int first = part, from = 0, to = 0, skip = 0, all = 1, n_parts = 1;
+        if (target) {
+            __shared__ int scan_s[NT / 64], found_s[2];
+            const int per = (p.B + NT - 1) / NT, b0 = threadIdx.x * per, b1 = min(b0 + per, p.B);
+            int mine = 0;                       // (the sum over all is at most 2^30: the caller keeps B * max_len below 2^36)
+            for (int x = b0; x < b1; ++x) mine += units_of(request_rows(p, x));
+            const int upto = block_scan<NT>(mine, scan_s, all);
+            n_parts = min(target, all);
+            from = (int)((long)part * all / n_parts);
+            to = (int)((long)(part + 1) * all / n_parts);
+            if (part < n_parts && upto > from && upto - mine <= from) {
+                int x = b0, before = upto - mine;
+                for (; x < b1 - 1; ++x) {
+                    const int n = units_of(request_rows(p, x));
+                    if (before + n > from) break;
+                    before += n;
+                }
+                found_s[0] = x;
+                found_s[1] = from - before;
+            }
+            __syncthreads();
+            first = found_s[0];
+            skip = found_s[1];
+        }
+        k = part;
+        parts = n_parts;
+        total = all;
+        b = __builtin_amdgcn_readfirstlane(first);
+        off = __builtin_amdgcn_readfirstlane(skip);
+        left = to - from;
+        at = from;
+        return part < (target ? n_parts : p.B);
     }
-    static __host__ __device__ long bytes(long n_items, int H, int depth, int B) { return n_items * H * (depth + 2) * 4 + (long)B * 8; }
+
+    // the next rows to do; items (of the first key head's workgroups): where the join finds request b
+    __device__ __forceinline__ PagedSegment next(const estts_paged_attention_args& p, int target, int2* items) {
+        const int rows = __builtin_amdgcn_readfirstlane(request_rows(p, b));
+        const int n = units_of(rows), take = target ? min(n - off, left) : n;
+        const PagedSegment s = {b, off * UNIT, min(rows, (off + take) * UNIT), 2 * k + (off == 0), take == n};
+        // unit x of the line is in part floor(((x + 1) parts - 1) / total)
+        if (target && off == 0 && items) items[b] = make_int2(k, take == n ? 1 : (int)((((long)at + n) * parts - 1) / total) - k + 1);
+        left -= take;
+        at += take;
+        off = 0;
+        ++b;
+        return s;
+    }
 };
 
-template <typename T, int DH, bool MASK>
-__global__ __launch_bounds__(ATT_WAVES * 64, 2) void paged_attention_kernel(const estts_paged_attention_args p, const int target, const int min_rows) {
-    constexpr bool F32 = sizeof(T) == 4;
-    constexpr int HALVES = F32 && DH == 128 ? 1 : 2;    // 16-row halves of a tile (float32 at depth 128: 64 registers of K and V are enough in flight)
-    constexpr int TILE = 16 * HALVES;
-    constexpr int NV = DH / 16;                         // consecutive features of a row of V per lane = tiles of 16 features
-    constexpr int PER_BLOCK = 64 / HALVES;              // tiles whose page entries the lanes of the wave hold at once
-    __shared__ __attribute__((aligned(16))) float o_s[ATT_WAVES][16][DH];
-    __shared__ float m_s[ATT_WAVES][16], l_s[ATT_WAVES][16];
+// scratch of a split call: per place and query head the unnormalised output (relative to its maximum), then (maximum, sum); per request
+// (part it begins in, number of parts it lies in)
+struct PagedScratch {
+    float* out; float2* ml; int2* items;
+    __host__ __device__ PagedScratch(void* ws, int target, int H, int depth) {
+        out = static_cast<float*>(ws);
+        ml = reinterpret_cast<float2*>(out + 2L * target * H * depth);
+        items = reinterpret_cast<int2*>(ml + 2L * target * H);
+    }
+    static __host__ __device__ long bytes(int target, int H, int depth, int B) { return 2L * target * H * (depth + 2) * 4 + (long)B * 8; }
+};
 
-    const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    // query groups of one key head next to each other on one XCD (workgroups whose numbers agree mod 8), whose L2 then holds the rows
-    const int group = p.H / p.kv_heads, n_group = (group + 15) >> 4;
-    int unit = blockIdx.x, part = 0;
-    if (n_group > 1) {
-        const int k = unit >> 3;
-        part = k % n_group;
-        unit = (k / n_group) * 8 + (unit & 7);
-    }
-    const int item = unit / p.kv_heads, hk = unit - item * p.kv_heads;
-    const int n_items = target ? target + p.B : p.B;
-    if (item >= n_items) return;
-    const PagedWork w = find_work(p, item, target, min_rows);
-    if (!w.any) return;
-    const int b = __builtin_amdgcn_readfirstlane(w.b), begin = __builtin_amdgcn_readfirstlane(w.begin), end = __builtin_amdgcn_readfirstlane(w.end);
-    const int heads = min(16, group - part * 16);       // query heads of this workgroup
-    const int h0 = hk * group + part * 16;
+// A wave's walk over its tiles t = wave, wave + NW, ... of rows [begin, end): where the 16-row halves of a tile lie in the caches.  A half
+// lies in one page (page sizes are multiples of 16), so that its place is one number for the whole wave; the lanes hold the places of
+// the next 64 halves, the table entries of the 64 after them are on their way.
+template <int HALVES, int NW>
+struct PageWalk {
+    static constexpr int TILE = 16 * HALVES, PER_BLOCK = 64 / HALVES;
+    const int* table;
+    long s_page, s_row;                                 // in bytes
+    int page, n_pages, max_len, begin, wave, lane;
+    int entry, next_entry, at_lo, at_hi;                // of this lane's half: its page, its byte offset (negative: no such page)
+    long at[HALVES];                                    // of the tile last located
+    bool ok[HALVES];
 
-    // ---- queries
-    const float qs = p.scale * 1.4426950408889634f;
-    const bool live = i < heads;
-    const float* qp = p.q + b * p.ldq + (long)(h0 + (live ? i : 0)) * DH;
-    constexpr int QV = F32 ? DH / 4 : DH / 4;           // elements of the query per lane
-    float qx[QV];
-#pragma unroll
-    for (int s = 0; s < QV / 4; ++s) {
-        // float32: step s of 16 features, lane g has 4g .. 4g+3; else step s / 2 of 32 features, lane g has 8g .. 8g+7
-        const float4 v = *reinterpret_cast<const float4*>(qp + (F32 ? 16 * s + 4 * g : 32 * (s >> 1) + 8 * g + 4 * (s & 1)));
-        qx[4 * s] = live ? v.x * qs : 0.0f;
-        qx[4 * s + 1] = live ? v.y * qs : 0.0f;
-        qx[4 * s + 2] = live ? v.z * qs : 0.0f;
-        qx[4 * s + 3] = live ? v.w * qs : 0.0f;
+    __device__ __forceinline__ PageWalk(const estts_paged_attention_args& p, int b, int begin_, int wave_, int esize)
+        : table(p.block_table + b * p.ld_table), s_page(p.s_page * esize), s_row(p.s_row * esize), page(p.page), n_pages(p.n_pages),
+          max_len(p.max_len), begin(begin_), wave(wave_), lane(threadIdx.x & 63) {
+        entry = entry_of(0);
+        next_entry = entry_of(1);
+        place(0);
     }
-    float unscale = 1.0f;                               // what the scores are multiplied with (float16: undoes the query's power of two)
-    if constexpr (!F32 && Kv16<T>::PIECES == 2) {
-        float top = 0.0f;
-#pragma unroll
-        for (int e = 0; e < QV; ++e) top = fmaxf(top, fabsf(qx[e]));
-        top = fmaxf(top, lane_xor16(top));
-        top = fmaxf(top, lane_xor32(top));
-        const int ex = max((int)(__builtin_bit_cast(uint32_t, top) >> 23), 14);
-        const float up = __builtin_bit_cast(float, (267 - ex) << 23);
-        unscale = __builtin_bit_cast(float, (ex - 13) << 23);
-#pragma unroll
-        for (int e = 0; e < QV; ++e) qx[e] *= up;
+    // first row of half lane % HALVES of tile number block * PER_BLOCK + lane / HALVES
+    __device__ __forceinline__ int half_row(int block) const {
+        return begin + ((block * PER_BLOCK + lane / HALVES) * NW + wave) * TILE + 16 * (lane % HALVES);
     }
-    [[maybe_unused]] typename Kv16<typename std::conditional<F32, __bf16, T>::type>::Frag qf[F32 ? 1 : DH / 32][3];
-    if constexpr (!F32) {
-#pragma unroll
-        for (int s = 0; s < DH / 32; ++s) {
-            float t[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) t[e] = qx[8 * s + e];
-            typename Kv16<T>::Frag f[Kv16<T>::PIECES];
-            split_pieces<T>(t, f);
-#pragma unroll
-            for (int n = 0; n < Kv16<T>::PIECES; ++n) qf[s][n] = f[n];
-        }
-    }
-
-    // ---- the wave's tiles: t = wave, wave + 4, ... of [begin, end)
-    const int n_tiles = (end - begin + TILE - 1) / TILE;
-    const int n_mine = __builtin_amdgcn_readfirstlane(n_tiles > wave ? (n_tiles - wave + ATT_WAVES - 1) / ATT_WAVES : 0);
-    const int* table = p.block_table + b * p.ld_table;
-    const char* kbase = static_cast<const char*>(p.k_cache) + hk * p.s_head * (long)sizeof(T);
-    const char* vbase = static_cast<const char*>(p.v_cache) + hk * p.s_head * (long)sizeof(T);
-    const int row_bytes = (int)(p.s_row * (long)sizeof(T));
-    // first row of half (lane % HALVES) of the wave's tile number block * PER_BLOCK + lane / HALVES; a half lies in one page
-    auto half_row = [&](int block) { return begin + ((block * PER_BLOCK + lane / HALVES) * ATT_WAVES + wave) * TILE + (HALVES == 2 ? 16 * (lane & 1) : 0); };
-    auto page_entry = [&](int block) { const int r = half_row(block); return r < end ? table[r / p.page] : -1; };
-    int entry = page_entry(0), next_entry = page_entry(1);
-    int at_lo, at_hi;                                   // byte offset of this lane's half in the caches, -1 where there is no such row or page
-    auto place = [&](int block) {
+    // (bounded by max_len, which the host knows, not by the length: the table and the lengths are read side by side)
+    __device__ __forceinline__ int entry_of(int block) const { return table[min(half_row(block), max_len - 1) / page]; }
+    __device__ __forceinline__ void place(int block) {
         const int r = half_row(block);
-        const bool ok = entry >= 0 && entry < p.n_pages;
-        const long at = ok ? ((long)entry * p.s_page + (long)(r % p.page) * p.s_row) * (long)sizeof(T) : -1L;
-        at_lo = (int)(at & 0xFFFFFFFFL);
-        at_hi = (int)(at >> 32);
-    };
-    place(0);
-
-    // registers of a tile
-    constexpr int KL = F32 ? DH / 16 : DH / 32;         // 16-byte loads of K per half and lane
-    constexpr int VW = NV * (int)sizeof(T) / 4;         // dwords of V per row and lane
-    int4 kr[HALVES][KL];
-    int vr[HALVES][4][VW];
-    [[maybe_unused]] float mk[HALVES][4];
-    const int k_lane = i * row_bytes + 16 * g;
-    const int v_lane = 4 * g * row_bytes + i * NV * (int)sizeof(T);
-    long half_at[HALVES];
-    bool half_ok[HALVES];
-    auto locate = [&](int it) {                         // of tile `it` of the wave
+        const bool there = entry >= 0 && entry < n_pages && r < max_len;
+        const long x = there ? entry * s_page + (long)(r % page) * s_row : -1L;
+        at_lo = (int)(x & 0xFFFFFFFFL);
+        at_hi = (int)(x >> 32);
+    }
+    // go to tile number it of the wave, the one after the last or the last again
+    __device__ __forceinline__ void locate(int it, bool next) {
+        if (next && it % PER_BLOCK == 0) {
+            entry = next_entry;
+            place(it / PER_BLOCK);
+            next_entry = entry_of(it / PER_BLOCK + 1);
+        }
         const int k = it % PER_BLOCK;
 #pragma unroll
         for (int s = 0; s < HALVES; ++s) {
             const int lo = __builtin_amdgcn_readlane(at_lo, k * HALVES + s), hi = __builtin_amdgcn_readlane(at_hi, k * HALVES + s);
-            half_ok[s] = hi >= 0;
-            half_at[s] = hi >= 0 ? (long)(((unsigned long)(unsigned)hi << 32) | (unsigned)lo) : 0;       // (row 0 of page 0 is always there)
-        }
-    };
-    auto load_k = [&](int it) {
-#pragma unroll
-        for (int s = 0; s < HALVES; ++s) {
-            const char* at = kbase + half_at[s];
-#pragma unroll
-            for (int x = 0; x < KL; ++x) kr[s][x] = *reinterpret_cast<const int4*>(at + (unsigned)(k_lane + 64 * x));
-        }
-        if constexpr (MASK) {
-            const float* mrow = p.key_mask + b * p.mask_sb;
-            const int r0 = begin + (it * ATT_WAVES + wave) * TILE + 4 * g;
-#pragma unroll
-            for (int s = 0; s < HALVES; ++s)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) mk[s][j] = mrow[min(r0 + 16 * s + j, end - 1) * p.mask_ss];
-        }
-    };
-    auto load_v = [&](const long (&at_half)[HALVES]) {
-#pragma unroll
-        for (int s = 0; s < HALVES; ++s) {
-            const char* at = vbase + at_half[s];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const char* a = at + (unsigned)(v_lane + j * row_bytes);
-                if constexpr (VW >= 4) {
-#pragma unroll
-                    for (int x = 0; x < VW / 4; ++x) {
-                        const int4 t = *reinterpret_cast<const int4*>(a + 16 * x);
-                        vr[s][j][4 * x] = t.x; vr[s][j][4 * x + 1] = t.y; vr[s][j][4 * x + 2] = t.z; vr[s][j][4 * x + 3] = t.w;
-                    }
-                } else if constexpr (VW == 2) {
-                    const int2 t = *reinterpret_cast<const int2*>(a);
-                    vr[s][j][0] = t.x; vr[s][j][VW - 1] = t.y;
-                } else {
-                    vr[s][j][0] = *reinterpret_cast<const int*>(a);
-                }
-            }
-        }
-    };
-
-    f32x4 o[NV];
-#pragma unroll
-    for (int e = 0; e < NV; ++e) o[e] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-    float m = -INFINITY, l = 0.0f;                      // of query i; l: this lane's rows only
-    constexpr float LIFT = !F32 && sizeof(T) == 2 && std::is_same<T, _Float16>::value ? 14.0f : 0.0f;
-
-    if (n_mine > 0) {
-        locate(0);
-        load_k(0);
-        load_v(half_at);
-        bool ok_now[HALVES];
-        for (int it = 0; it < n_mine; ++it) {
-#pragma unroll
-            for (int s = 0; s < HALVES; ++s) ok_now[s] = half_ok[s];
-            const int r0 = begin + (it * ATT_WAVES + wave) * TILE;
-            // scores
-            float sc[HALVES][4];
-            if constexpr (F32) {
-#pragma unroll
-                for (int s = 0; s < HALVES; ++s) {
-                    f32x4 a0 = {0.0f, 0.0f, 0.0f, 0.0f}, a1 = a0;
-#pragma unroll
-                    for (int x = 0; x < KL; ++x) {
-                        a0 = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, kr[s][x].x), qx[4 * x], a0, 0, 0, 0);
-                        a1 = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, kr[s][x].y), qx[4 * x + 1], a1, 0, 0, 0);
-                        a0 = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, kr[s][x].z), qx[4 * x + 2], a0, 0, 0, 0);
-                        a1 = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, kr[s][x].w), qx[4 * x + 3], a1, 0, 0, 0);
-                    }
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) sc[s][j] = a0[j] + a1[j];
-                }
-            } else {
-                f32x4 acc[HALVES][Kv16<T>::PIECES];
-#pragma unroll
-                for (int s = 0; s < HALVES; ++s)
-#pragma unroll
-                    for (int n = 0; n < Kv16<T>::PIECES; ++n) acc[s][n] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int x = 0; x < KL; ++x)
-#pragma unroll
-                    for (int n = 0; n < Kv16<T>::PIECES; ++n)
-#pragma unroll
-                        for (int s = 0; s < HALVES; ++s)
-                            acc[s][n] = Kv16<T>::mfma(__builtin_bit_cast(typename Kv16<T>::Frag, kr[s][x]), qf[x][n], acc[s][n]);
-#pragma unroll
-                for (int s = 0; s < HALVES; ++s)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        float t = acc[s][Kv16<T>::PIECES - 1][j];
-#pragma unroll
-                        for (int n = Kv16<T>::PIECES - 2; n >= 0; --n) t += acc[s][n][j];
-                        sc[s][j] = Kv16<T>::PIECES == 2 ? t * unscale : t;
-                    }
-            }
-            // rows that count: in range, in a page that exists, not masked
-            bool all_in = r0 + TILE <= end;
-#pragma unroll
-            for (int s = 0; s < HALVES; ++s) all_in = all_in && ok_now[s];
-            bool in[HALVES][4];
-#pragma unroll
-            for (int s = 0; s < HALVES; ++s)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    in[s][j] = ok_now[s] && r0 + 16 * s + 4 * g + j < end;
-                    if constexpr (MASK) in[s][j] = in[s][j] && mk[s][j] == 0.0f;
-                }
-            bool drop = !all_in;
-            if constexpr (MASK) {
-                bool mine = true;
-#pragma unroll
-                for (int s = 0; s < HALVES; ++s)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) mine = mine && in[s][j];
-                drop = __any(!mine);
-            }
-            // the next tile's keys, into the registers just read (the last tile again where there is none: the number of loads in
-            // flight stays the same on every path, so that no wait is longer than it has to be)
-            const int nx = min(it + 1, n_mine - 1);
-            if (nx % PER_BLOCK == 0 && nx != it) {
-                entry = next_entry;
-                place(nx / PER_BLOCK);
-                next_entry = page_entry(nx / PER_BLOCK + 1);
-            }
-            locate(nx);
-            load_k(nx);
-            if (drop) {
-#pragma unroll
-                for (int s = 0; s < HALVES; ++s)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        sc[s][j] = in[s][j] ? sc[s][j] : -INFINITY;
-#pragma unroll
-                        for (int x = 0; x < VW; ++x) vr[s][j][x] = in[s][j] ? vr[s][j][x] : 0;       // (0 x NaN would be NaN)
-                    }
-            }
-            // softmax step
-            float top = sc[0][0];
-#pragma unroll
-            for (int s = 0; s < HALVES; ++s)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) top = fmaxf(top, sc[s][j]);
-            top = fmaxf(top, lane_xor16(top));
-            top = fmaxf(top, lane_xor32(top));
-            if (__any(top > m)) {
-                const float m1 = fmaxf(m, top);
-                const float c = m1 == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - m1);
-                m = m1;
-                l *= c;
-#pragma unroll
-                for (int e = 0; e < NV; ++e)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) o[e][j] *= c;
-            }
-            const float base = (m == -INFINITY ? 0.0f : m) - LIFT;
-            float pw[8];
-#pragma unroll
-            for (int s = 0; s < HALVES; ++s)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    pw[4 * s + j] = __builtin_amdgcn_exp2f(sc[s][j] - base);
-                    l += pw[4 * s + j];
-                }
-            // output
-            if constexpr (F32) {
-#pragma unroll
-                for (int s = 0; s < HALVES; ++s)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-#pragma unroll
-                        for (int e = 0; e < NV; ++e)
-                            o[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, vr[s][j][e]), pw[4 * s + j], o[e], 0, 0, 0);
-            } else {
-                typename Kv16<T>::Frag pf[Kv16<T>::PIECES];
-                split_pieces<T>(pw, pf);
-#pragma unroll
-                for (int e = 0; e < NV; ++e) {
-                    int4 a;
-                    int* ap = reinterpret_cast<int*>(&a);
-#pragma unroll
-                    for (int d = 0; d < 4; ++d)         // slots 2d, 2d + 1: rows (half d / 2, 2 (d % 2)) and the next
-                        ap[d] = __builtin_amdgcn_perm(vr[d >> 1][2 * (d & 1) + 1][e >> 1], vr[d >> 1][2 * (d & 1)][e >> 1], e & 1 ? 0x07060302u : 0x05040100u);
-                    const auto vf = __builtin_bit_cast(typename Kv16<T>::Frag, a);
-#pragma unroll
-                    for (int n = Kv16<T>::PIECES - 1; n >= 0; --n) o[e] = Kv16<T>::mfma(vf, pf[n], o[e]);
-                }
-            }
-            load_v(half_at);
+            ok[s] = hi >= 0;
+            at[s] = hi >= 0 ? (long)(((unsigned long)(unsigned)hi << 32) | (unsigned)lo) : 0;            // (row 0 of page 0 is always there)
         }
     }
+};
 
-    // ---- the waves' shares meet
-    l += lane_xor16(l);
-    l += lane_xor32(l);
-    if (live) {
-        if (g == 0) { m_s[wave][i] = m; l_s[wave][i] = l; }
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int e = 0; e < NV; e += NV < 4 ? NV : 4) {
-                float* at = &o_s[wave][i][(4 * g + j) * NV + e];
-                if constexpr (NV >= 4) *reinterpret_cast<float4*>(at) = make_float4(o[e][j], o[e + 1][j], o[e + 2][j], o[e + 3][j]);
-                else *reinterpret_cast<float2*>(at) = make_float2(o[e][j], o[e + 1][j]);
-            }
+// what a workgroup works on: a request or a part of the line (`part`), key head hk, query heads h0 .. h0 + heads - 1 (at most MAXQ)
+template <int MAXQ>
+struct PagedUnit {
+    int part, hk, h0, heads;
+    __device__ __forceinline__ PagedUnit(const estts_paged_attention_args& p) {
+        // query groups of one key head next to each other on one XCD (workgroups whose numbers agree mod 8), whose L2 then holds the rows
+        const int group = p.H / p.kv_heads, n_group = (group + MAXQ - 1) / MAXQ;
+        int unit = blockIdx.x, q = 0;
+        if (n_group > 1) {
+            const int k = unit >> 3;
+            q = k % n_group;
+            unit = (k / n_group) * 8 + (unit & 7);
+        }
+        part = unit / p.kv_heads;
+        hk = unit - part * p.kv_heads;
+        heads = min(MAXQ, group - q * MAXQ);
+        h0 = hk * group + q * MAXQ;
     }
-    __syncthreads();
-    const PagedScratch ws(p.ws, n_items, p.H, DH);
-    if (target && w.split == 0 && unit % p.kv_heads == 0 && part == 0 && threadIdx.x == 0) ws.items[b] = make_int2(w.first, w.n_split);
-    for (int x = threadIdx.x; x < heads * DH; x += ATT_WAVES * 64) {
+};
+
+// The waves' shares (o_s, m_s, l_s in the LDS) meet; to ctx, or to the scratch where the segment is not a whole request.
+template <int NW, int MAXQ, int DH>
+__device__ __forceinline__ void join_waves(const estts_paged_attention_args& p, const PagedUnit<MAXQ>& u, const PagedSegment& seg, const PagedScratch& ws,
+                                           const float (*o_s)[MAXQ][DH], const float (*m_s)[MAXQ], const float (*l_s)[MAXQ]) {
+    for (int x = threadIdx.x; x < u.heads * DH; x += NW * 64) {
         const int h = x / DH, d = x % DH;
         float top = m_s[0][h];
 #pragma unroll
-        for (int v = 1; v < ATT_WAVES; ++v) top = fmaxf(top, m_s[v][h]);
+        for (int v = 1; v < NW; ++v) top = fmaxf(top, m_s[v][h]);
         const float base = top == -INFINITY ? 0.0f : top;
         float sum = 0.0f, acc = 0.0f;
 #pragma unroll
-        for (int v = 0; v < ATT_WAVES; ++v) {
+        for (int v = 0; v < NW; ++v) {
             const float c = __builtin_amdgcn_exp2f(m_s[v][h] - base);
             sum = fmaf(l_s[v][h], c, sum);
             acc = fmaf(o_s[v][h][d], c, acc);
         }
-        if (w.n_split == 1) {
-            p.ctx[b * p.ldo + (long)(h0 + h) * DH + d] = sum == 0.0f ? 0.0f : acc / sum;
+        if (seg.whole) {
+            p.ctx[seg.b * p.ldo + (long)(u.h0 + h) * DH + d] = sum == 0.0f ? 0.0f : acc / sum;
         } else {
-            const long at = (long)item * p.H + h0 + h;
+            const long at = (long)seg.place * p.H + u.h0 + h;
             ws.out[at * DH + d] = acc;
             if (d == 0) ws.ml[at] = make_float2(top, sum);
         }
     }
 }
 
-// The splits of a request meet: one workgroup per (query head, request), its waves take every fourth split.
+template <typename T, int DH, bool MASK, int NW>
+__global__ __launch_bounds__(NW * 64, 2) void paged_attention_kernel(const estts_paged_attention_args p, const int target) {
+    constexpr bool F32 = sizeof(T) == 4;
+    constexpr int HALVES = tile_halves(DH, sizeof(T));
+    constexpr int TILE = 16 * HALVES;
+    constexpr int NV = DH / 16;                         // consecutive features of a row of V per lane = tiles of 16 features
+    __shared__ __attribute__((aligned(16))) float o_s[NW][16][DH];
+    __shared__ float m_s[NW][16], l_s[NW][16];
+
+    const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const PagedUnit<16> u(p);
+    const int heads = u.heads, h0 = u.h0;
+    const PagedScratch ws(p.ws, target, p.H, DH);
+    PagedPart<NW * 64, TILE * NW> part;
+    if (!part.find(p, u.part, target)) return;
+    do {
+        const PagedSegment seg = part.next(p, target, h0 == 0 && threadIdx.x == 0 ? ws.items : nullptr);
+        const int b = seg.b, begin = seg.begin, end = seg.end;
+        PageWalk<HALVES, NW> walk(p, b, begin, wave, sizeof(T));
+
+        // ---- queries
+        const float qs = p.scale * 1.4426950408889634f;
+        const bool live = i < heads;
+        const float* qp = p.q + b * p.ldq + (long)(h0 + (live ? i : 0)) * DH;
+        constexpr int QV = F32 ? DH / 4 : DH / 4;           // elements of the query per lane
+        float qx[QV];
+#pragma unroll
+        for (int s = 0; s < QV / 4; ++s) {
+            // float32: step s of 16 features, lane g has 4g .. 4g+3; else step s / 2 of 32 features, lane g has 8g .. 8g+7
+            const float4 v = *reinterpret_cast<const float4*>(qp + (F32 ? 16 * s + 4 * g : 32 * (s >> 1) + 8 * g + 4 * (s & 1)));
+            qx[4 * s] = live ? v.x * qs : 0.0f;
+            qx[4 * s + 1] = live ? v.y * qs : 0.0f;
+            qx[4 * s + 2] = live ? v.z * qs : 0.0f;
+            qx[4 * s + 3] = live ? v.w * qs : 0.0f;
+        }
+        float unscale = 1.0f;                               // what the scores are multiplied with (float16: undoes the query's power of two)
+        if constexpr (!F32 && Kv16<T>::PIECES == 2) {
+            float top = 0.0f;
+#pragma unroll
+            for (int e = 0; e < QV; ++e) top = fmaxf(top, fabsf(qx[e]));
+            top = fmaxf(top, lane_xor16(top));
+            top = fmaxf(top, lane_xor32(top));
+            const int ex = max((int)(__builtin_bit_cast(uint32_t, top) >> 23), 14);
+            const float up = __builtin_bit_cast(float, (267 - ex) << 23);
+            unscale = __builtin_bit_cast(float, (ex - 13) << 23);
+#pragma unroll
+            for (int e = 0; e < QV; ++e) qx[e] *= up;
+        }
+        [[maybe_unused]] typename Kv16<typename std::conditional<F32, __bf16, T>::type>::Frag qf[F32 ? 1 : DH / 32][3];
+        if constexpr (!F32) {
+#pragma unroll
+            for (int s = 0; s < DH / 32; ++s) {
+                float t[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) t[e] = qx[8 * s + e];
+                typename Kv16<T>::Frag f[Kv16<T>::PIECES];
+                split_pieces<T>(t, f);
+#pragma unroll
+                for (int n = 0; n < Kv16<T>::PIECES; ++n) qf[s][n] = f[n];
+            }
+        }
+
+        // ---- the wave's tiles
+        const int n_tiles = (end - begin + TILE - 1) / TILE;
+        const int n_mine = __builtin_amdgcn_readfirstlane(n_tiles > wave ? (n_tiles - wave + NW - 1) / NW : 0);
+        const char* kbase = static_cast<const char*>(p.k_cache) + u.hk * p.s_head * (long)sizeof(T);
+        const char* vbase = static_cast<const char*>(p.v_cache) + u.hk * p.s_head * (long)sizeof(T);
+        const int row_bytes = (int)(p.s_row * (long)sizeof(T));
+
+        // registers of a tile
+        constexpr int KL = F32 ? DH / 16 : DH / 32;         // 16-byte loads of K per half and lane
+        constexpr int VW = NV * (int)sizeof(T) / 4;         // dwords of V per row and lane
+        int4 kr[HALVES][KL];
+        int vr[HALVES][4][VW];
+        [[maybe_unused]] float mk[HALVES][4];
+        const int k_lane = i * row_bytes + 16 * g;
+        const int v_lane = 4 * g * row_bytes + i * NV * (int)sizeof(T);
+        auto load_k = [&](int it) {
+#pragma unroll
+            for (int s = 0; s < HALVES; ++s) {
+                const char* at = kbase + walk.at[s];
+#pragma unroll
+                for (int x = 0; x < KL; ++x) kr[s][x] = *reinterpret_cast<const int4*>(at + (unsigned)(k_lane + 64 * x));
+            }
+            if constexpr (MASK) {
+                const float* mrow = p.key_mask + b * p.mask_sb;
+                const int r0 = begin + (it * NW + wave) * TILE + 4 * g;
+#pragma unroll
+                for (int s = 0; s < HALVES; ++s)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) mk[s][j] = mrow[min(r0 + 16 * s + j, end - 1) * p.mask_ss];
+            }
+        };
+        auto load_v = [&]() {
+#pragma unroll
+            for (int s = 0; s < HALVES; ++s) {
+                const char* at = vbase + walk.at[s];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const char* a = at + (unsigned)(v_lane + j * row_bytes);
+                    if constexpr (VW >= 4) {
+#pragma unroll
+                        for (int x = 0; x < VW / 4; ++x) {
+                            const int4 t = *reinterpret_cast<const int4*>(a + 16 * x);
+                            vr[s][j][4 * x] = t.x; vr[s][j][4 * x + 1] = t.y; vr[s][j][4 * x + 2] = t.z; vr[s][j][4 * x + 3] = t.w;
+                        }
+                    } else if constexpr (VW == 2) {
+                        const int2 t = *reinterpret_cast<const int2*>(a);
+                        vr[s][j][0] = t.x; vr[s][j][VW - 1] = t.y;
+                    } else {
+                        vr[s][j][0] = *reinterpret_cast<const int*>(a);
+                    }
+                }
+            }
+        };
+
+        f32x4 o[NV];
+#pragma unroll
+        for (int e = 0; e < NV; ++e) o[e] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+        float m = -INFINITY, l = 0.0f;                      // of query i; l: this lane's rows only
+        constexpr float LIFT = !F32 && sizeof(T) == 2 && std::is_same<T, _Float16>::value ? 14.0f : 0.0f;
+
+        if (n_mine > 0) {
+            walk.locate(0, false);
+            load_k(0);
+            load_v();
+            bool ok_now[HALVES];
+            for (int it = 0; it < n_mine; ++it) {
+#pragma unroll
+                for (int s = 0; s < HALVES; ++s) ok_now[s] = walk.ok[s];
+                const int r0 = begin + (it * NW + wave) * TILE;
+                // scores
+                float sc[HALVES][4];
+                if constexpr (F32) {
+#pragma unroll
+                    for (int s = 0; s < HALVES; ++s) {
+                        f32x4 a0 = {0.0f, 0.0f, 0.0f, 0.0f}, a1 = a0;
+#pragma unroll
+                        for (int x = 0; x < KL; ++x) {
+                            a0 = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, kr[s][x].x), qx[4 * x], a0, 0, 0, 0);
+                            a1 = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, kr[s][x].y), qx[4 * x + 1], a1, 0, 0, 0);
+                            a0 = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, kr[s][x].z), qx[4 * x + 2], a0, 0, 0, 0);
+                            a1 = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, kr[s][x].w), qx[4 * x + 3], a1, 0, 0, 0);
+                        }
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) sc[s][j] = a0[j] + a1[j];
+                    }
+                } else {
+                    f32x4 acc[HALVES][Kv16<T>::PIECES];
+#pragma unroll
+                    for (int s = 0; s < HALVES; ++s)
+#pragma unroll
+                        for (int n = 0; n < Kv16<T>::PIECES; ++n) acc[s][n] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int x = 0; x < KL; ++x)
+#pragma unroll
+                        for (int n = 0; n < Kv16<T>::PIECES; ++n)
+#pragma unroll
+                            for (int s = 0; s < HALVES; ++s)
+                                acc[s][n] = Kv16<T>::mfma(__builtin_bit_cast(typename Kv16<T>::Frag, kr[s][x]), qf[x][n], acc[s][n]);
+#pragma unroll
+                    for (int s = 0; s < HALVES; ++s)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            float t = acc[s][Kv16<T>::PIECES - 1][j];
+#pragma unroll
+                            for (int n = Kv16<T>::PIECES - 2; n >= 0; --n) t += acc[s][n][j];
+                            sc[s][j] = Kv16<T>::PIECES == 2 ? t * unscale : t;
+                        }
+                }
+                // rows that count: in range, in a page that exists, not masked
+                bool all_in = r0 + TILE <= end;
+#pragma unroll
+                for (int s = 0; s < HALVES; ++s) all_in = all_in && ok_now[s];
+                bool in[HALVES][4];
+#pragma unroll
+                for (int s = 0; s < HALVES; ++s)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        in[s][j] = ok_now[s] && r0 + 16 * s + 4 * g + j < end;
+                        if constexpr (MASK) in[s][j] = in[s][j] && mk[s][j] == 0.0f;
+                    }
+                bool drop = !all_in;
+                if constexpr (MASK) {
+                    bool mine = true;
+#pragma unroll
+                    for (int s = 0; s < HALVES; ++s)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) mine = mine && in[s][j];
+                    drop = __any(!mine);
+                }
+                // the next tile's keys, into the registers just read (the last tile again where there is none: the number of loads in
+                // flight stays the same on every path, so that no wait is longer than it has to be)
+                const int nx = min(it + 1, n_mine - 1);
+                walk.locate(nx, nx != it);
+                load_k(nx);
+                if (drop) {
+#pragma unroll
+                    for (int s = 0; s < HALVES; ++s)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            sc[s][j] = in[s][j] ? sc[s][j] : -INFINITY;
+#pragma unroll
+                            for (int x = 0; x < VW; ++x) vr[s][j][x] = in[s][j] ? vr[s][j][x] : 0;       // (0 x NaN would be NaN)
+                        }
+                }
+                // softmax step
+                float top = sc[0][0];
+#pragma unroll
+                for (int s = 0; s < HALVES; ++s)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) top = fmaxf(top, sc[s][j]);
+                top = fmaxf(top, lane_xor16(top));
+                top = fmaxf(top, lane_xor32(top));
+                if (__any(top > m)) {
+                    const float m1 = fmaxf(m, top);
+                    const float c = m1 == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - m1);
+                    m = m1;
+                    l *= c;
+#pragma unroll
+                    for (int e = 0; e < NV; ++e)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) o[e][j] *= c;
+                }
+                const float base = (m == -INFINITY ? 0.0f : m) - LIFT;
+                float pw[8];
+#pragma unroll
+                for (int s = 0; s < HALVES; ++s)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        pw[4 * s + j] = __builtin_amdgcn_exp2f(sc[s][j] - base);
+                        l += pw[4 * s + j];
+                    }
+                // output
+                if constexpr (F32) {
+#pragma unroll
+                    for (int s = 0; s < HALVES; ++s)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+#pragma unroll
+                            for (int e = 0; e < NV; ++e)
+                                o[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, vr[s][j][e]), pw[4 * s + j], o[e], 0, 0, 0);
+                } else {
+                    typename Kv16<T>::Frag pf[Kv16<T>::PIECES];
+                    split_pieces<T>(pw, pf);
+#pragma unroll
+                    for (int e = 0; e < NV; ++e) {
+                        int4 a;
+                        int* ap = reinterpret_cast<int*>(&a);
+#pragma unroll
+                        for (int d = 0; d < 4; ++d)         // slots 2d, 2d + 1: rows (half d / 2, 2 (d % 2)) and the next
+                            ap[d] = __builtin_amdgcn_perm(vr[d >> 1][2 * (d & 1) + 1][e >> 1], vr[d >> 1][2 * (d & 1)][e >> 1], e & 1 ? 0x07060302u : 0x05040100u);
+                        const auto vf = __builtin_bit_cast(typename Kv16<T>::Frag, a);
+#pragma unroll
+                        for (int n = Kv16<T>::PIECES - 1; n >= 0; --n) o[e] = Kv16<T>::mfma(vf, pf[n], o[e]);
+                    }
+                }
+                load_v();
+            }
+        }
+
+        // ---- the waves' shares meet
+        l += lane_xor16(l);
+        l += lane_xor32(l);
+        if (live) {
+            if (g == 0) { m_s[wave][i] = m; l_s[wave][i] = l; }
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int e = 0; e < NV; e += NV < 4 ? NV : 4) {
+                    float* at = &o_s[wave][i][(4 * g + j) * NV + e];
+                    if constexpr (NV >= 4) *reinterpret_cast<float4*>(at) = make_float4(o[e][j], o[e + 1][j], o[e + 2][j], o[e + 3][j]);
+                    else *reinterpret_cast<float2*>(at) = make_float2(o[e][j], o[e + 1][j]);
+                }
+        }
+        __syncthreads();
+        join_waves<NW, 16, DH>(p, u, seg, ws, o_s, m_s, l_s);
+        if (part.left > 0) __syncthreads();         // (before the next segment's shares)
+    } while (part.left > 0);
+}
+
+// The same for float32 pages and a key head that only one or two query heads read (NQ): most columns of a matrix tile would be empty
+// and its 64 float32 matrix instructions a tile (2048 cycles) would set the time of a short request.  On the vector ALU a tile
+// is 64 multiply-adds, 32 data-parallel additions and 8 exponentials a lane and query (some 700 cycles).  Lane (i, g) holds the
+// depth/16 features from i depth/16 on of rows 4g + j of a half, of K as of V; the sixteen lanes of a row add up its score.
+// One request of 1000 rows, 4 key heads of 64 / 128, matrix cores / here: one query head each 13.4 / 8.0 and 22.2 / 10.7 us, two 13.6 / 10.6
+// and 22.4 / 14.8; 64 such requests, bound by memory: 26.5 / 25.4 and 48.3 / 47.2 us (5.3 and 5.7 TB/s).
+__device__ __forceinline__ float row_sum(float v) {     // over the 16 lanes of a row, to all of them
+#define ESTTS_ROW_STEP(ctrl) v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), ctrl, 0xf, 0xf, false))
+    ESTTS_ROW_STEP(0xB1);        // quad_perm [1, 0, 3, 2]
+    ESTTS_ROW_STEP(0x4E);        // quad_perm [2, 3, 0, 1]
+    ESTTS_ROW_STEP(0x141);       // row_half_mirror
+    ESTTS_ROW_STEP(0x140);       // row_mirror
+#undef ESTTS_ROW_STEP
+    return v;
+}
+
+template <int DH, bool MASK, int NQ, int NW>
+__global__ __launch_bounds__(NW * 64, 2) void paged_attention_few_kernel(const estts_paged_attention_args p, const int target) {
+    constexpr int HALVES = tile_halves(DH, 4), TILE = 16 * HALVES, NV = DH / 16;
+    __shared__ __attribute__((aligned(16))) float o_s[NW][NQ][DH];
+    __shared__ float m_s[NW][NQ], l_s[NW][NQ];
+    const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const PagedUnit<NQ> u(p);
+    const PagedScratch ws(p.ws, target, p.H, DH);
+    PagedPart<NW * 64, TILE * NW> part;
+    if (!part.find(p, u.part, target)) return;
+    do {
+        const PagedSegment seg = part.next(p, target, u.h0 == 0 && threadIdx.x == 0 ? ws.items : nullptr);
+        const int b = seg.b, begin = seg.begin, end = seg.end;
+        PageWalk<HALVES, NW> walk(p, b, begin, wave, 4);
+        const float qs = p.scale * 1.4426950408889634f;
+        float qx[NQ][NV];
+#pragma unroll
+        for (int n = 0; n < NQ; ++n)
+#pragma unroll
+            for (int e = 0; e < NV; ++e) qx[n][e] = p.q[b * p.ldq + (long)(u.h0 + min(n, u.heads - 1)) * DH + i * NV + e] * qs;
+        const int n_tiles = (end - begin + TILE - 1) / TILE;
+        const int n_mine = __builtin_amdgcn_readfirstlane(n_tiles > wave ? (n_tiles - wave + NW - 1) / NW : 0);
+        const char* kbase = static_cast<const char*>(p.k_cache) + u.hk * p.s_head * 4;
+        const char* vbase = static_cast<const char*>(p.v_cache) + u.hk * p.s_head * 4;
+        const int row_bytes = (int)(p.s_row * 4);
+        const int lane_at = 4 * g * row_bytes + i * NV * 4;
+
+        float kr[HALVES][4][NV], vr[HALVES][4][NV];
+        [[maybe_unused]] float mk[HALVES][4];
+        auto load = [&](const char* base, float (&r)[HALVES][4][NV]) {
+#pragma unroll
+            for (int s = 0; s < HALVES; ++s)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const char* a = base + walk.at[s] + (unsigned)(lane_at + j * row_bytes);
+                    if constexpr (NV == 2) {
+                        const float2 t = *reinterpret_cast<const float2*>(a);
+                        r[s][j][0] = t.x; r[s][j][1] = t.y;
+                    } else {
+#pragma unroll
+                        for (int x = 0; x < NV; x += 4) {
+                            const float4 t = *reinterpret_cast<const float4*>(a + 4 * x);
+                            r[s][j][x] = t.x; r[s][j][x + 1] = t.y; r[s][j][x + 2] = t.z; r[s][j][x + 3] = t.w;
+                        }
+                    }
+                }
+        };
+        auto load_mask = [&](int it) {
+            if constexpr (MASK) {
+                const float* mrow = p.key_mask + b * p.mask_sb;
+                const int r0 = begin + (it * NW + wave) * TILE + 4 * g;
+#pragma unroll
+                for (int s = 0; s < HALVES; ++s)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) mk[s][j] = mrow[min(r0 + 16 * s + j, end - 1) * p.mask_ss];
+            }
+        };
+        float m[NQ], l[NQ], o[NQ][NV];
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {
+            m[n] = -INFINITY;
+            l[n] = 0.0f;
+#pragma unroll
+            for (int e = 0; e < NV; ++e) o[n][e] = 0.0f;
+        }
+        if (n_mine > 0) {
+            walk.locate(0, false);
+            load(kbase, kr);
+            load_mask(0);
+            load(vbase, vr);
+            for (int it = 0; it < n_mine; ++it) {
+                const int r0 = begin + (it * NW + wave) * TILE;
+                bool ok_now[HALVES], all_in = r0 + TILE <= end;
+#pragma unroll
+                for (int s = 0; s < HALVES; ++s) {
+                    ok_now[s] = walk.ok[s];
+                    all_in = all_in && ok_now[s];
+                }
+                float sc[NQ][HALVES][4];
+#pragma unroll
+                for (int n = 0; n < NQ; ++n)
+#pragma unroll
+                    for (int s = 0; s < HALVES; ++s)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            float t = kr[s][j][0] * qx[n][0];
+#pragma unroll
+                            for (int e = 1; e < NV; ++e) t = fmaf(kr[s][j][e], qx[n][e], t);
+                            sc[n][s][j] = row_sum(t);
+                        }
+                bool in[HALVES][4], mine = true;
+#pragma unroll
+                for (int s = 0; s < HALVES; ++s)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        in[s][j] = ok_now[s] && r0 + 16 * s + 4 * g + j < end;
+                        if constexpr (MASK) in[s][j] = in[s][j] && mk[s][j] == 0.0f;
+                        mine = mine && in[s][j];
+                    }
+                const bool drop = MASK ? (bool)__any(!mine) : !all_in;
+                const int nx = min(it + 1, n_mine - 1);
+                walk.locate(nx, nx != it);
+                load(kbase, kr);
+                load_mask(nx);
+                if (drop) {
+#pragma unroll
+                    for (int s = 0; s < HALVES; ++s)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+#pragma unroll
+                            for (int n = 0; n < NQ; ++n) sc[n][s][j] = in[s][j] ? sc[n][s][j] : -INFINITY;
+#pragma unroll
+                            for (int e = 0; e < NV; ++e) vr[s][j][e] = in[s][j] ? vr[s][j][e] : 0.0f;
+                        }
+                }
+#pragma unroll
+                for (int n = 0; n < NQ; ++n) {
+                    float top = sc[n][0][0];
+#pragma unroll
+                    for (int s = 0; s < HALVES; ++s)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) top = fmaxf(top, sc[n][s][j]);
+                    top = fmaxf(top, lane_xor16(top));
+                    top = fmaxf(top, lane_xor32(top));
+                    const float m1 = fmaxf(m[n], top);
+                    const float base = m1 == -INFINITY ? 0.0f : m1;
+                    const float c = __builtin_amdgcn_exp2f(m[n] - base);
+                    m[n] = m1;
+                    l[n] *= c;
+#pragma unroll
+                    for (int e = 0; e < NV; ++e) o[n][e] *= c;
+#pragma unroll
+                    for (int s = 0; s < HALVES; ++s)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const float w = __builtin_amdgcn_exp2f(sc[n][s][j] - base);
+                            l[n] += w;
+#pragma unroll
+                            for (int e = 0; e < NV; ++e) o[n][e] = fmaf(w, vr[s][j][e], o[n][e]);
+                        }
+                }
+                load(vbase, vr);
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {
+            l[n] += lane_xor16(l[n]);
+            l[n] += lane_xor32(l[n]);
+            if (lane == 0) { m_s[wave][n] = m[n]; l_s[wave][n] = l[n]; }
+#pragma unroll
+            for (int e = 0; e < NV; ++e) {
+                o[n][e] += lane_xor16(o[n][e]);
+                o[n][e] += lane_xor32(o[n][e]);
+                if (g == 0) o_s[wave][n][i * NV + e] = o[n][e];
+            }
+        }
+        __syncthreads();
+        join_waves<NW, NQ, DH>(p, u, seg, ws, o_s, m_s, l_s);
+        if (part.left > 0) __syncthreads();         // (before the next segment's shares)
+    } while (part.left > 0);
+}
+
+// The parts of a request meet: one workgroup per (query head, request).  Each of its eight half-waves takes every eighth part, four at a
+// time and each read once, with a running maximum of its own; then they meet in the LDS.
 template <int DH>
-__global__ __launch_bounds__(256) void paged_join_kernel(const estts_paged_attention_args p, const int n_items) {
-    __shared__ float acc_s[4][DH], sum_s[4];
+__global__ __launch_bounds__(256) void paged_join_kernel(const estts_paged_attention_args p, const int target) {
+    __shared__ float acc_s[8][DH], m_s[8], l_s[8];
     const int h = blockIdx.x, b = blockIdx.y;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const PagedScratch ws(p.ws, n_items, p.H, DH);
+    const int lane = threadIdx.x & 31, team = threadIdx.x >> 5;
+    const PagedScratch ws(p.ws, target, p.H, DH);
     const int2 it = ws.items[b];
     if (it.y <= 1) return;
-    const float2* ml = ws.ml + (long)it.x * p.H + h;
-    float top = -INFINITY;
-    for (int s = lane; s < it.y; s += 64) top = fmaxf(top, ml[(long)s * p.H].x);
-    top = wave_max(top);
-    const float base = top == -INFINITY ? 0.0f : top;
-    constexpr int PER = DH / 32;                      // features per lane; the halves of a wave take different splits
-    const int f = (lane & 31) * PER;
-    float acc[PER] = {}, sum = 0.0f;
-    const float* out = ws.out + ((long)it.x * p.H + h) * DH + f;
-#pragma unroll 4
-    for (int s = 2 * wave + (lane >> 5); s < it.y; s += 8) {
-        const float2 v = ml[(long)s * p.H];
-        const float c = __builtin_amdgcn_exp2f(v.x - base);
-        sum = fmaf(v.y, c, sum);
+    constexpr int PER = DH / 32, STEP = 4;            // features per lane; parts in flight
+    float acc[PER] = {}, m = -INFINITY, l = 0.0f;
+    for (int s0 = team; s0 < it.y; s0 += 8 * STEP) {
+        float2 ml[STEP];
+        float x[STEP][PER];
 #pragma unroll
-        for (int e = 0; e < PER; ++e) acc[e] = fmaf(out[(long)s * p.H * DH + e], c, acc[e]);
-    }
-    sum += lane_xor32(sum);
+        for (int k = 0; k < STEP; ++k) {
+            // part it.x holds the request's beginning (place 2 it.x + 1), the others are at the even places after it
+            const int s = min(s0 + 8 * k, it.y - 1);
+            const long at = (long)(s == 0 ? 2 * it.x + 1 : 2 * (it.x + s)) * p.H + h;
+            ml[k] = ws.ml[at];
 #pragma unroll
-    for (int e = 0; e < PER; ++e) {
-        acc[e] += lane_xor32(acc[e]);
-        if (lane < 32) acc_s[wave][f + e] = acc[e];
+            for (int e = 0; e < PER; ++e) x[k][e] = ws.out[at * DH + lane * PER + e];
+        }
+        float top = m;
+#pragma unroll
+        for (int k = 0; k < STEP; ++k) {
+            if (s0 + 8 * k >= it.y) ml[k] = make_float2(-INFINITY, 0.0f);
+            top = fmaxf(top, ml[k].x);
+        }
+        const float base = top == -INFINITY ? 0.0f : top;
+        const float c0 = __builtin_amdgcn_exp2f(m - base);
+        l *= c0;
+#pragma unroll
+        for (int e = 0; e < PER; ++e) acc[e] *= c0;
+#pragma unroll
+        for (int k = 0; k < STEP; ++k) {
+            const float c = __builtin_amdgcn_exp2f(ml[k].x - base);
+            l = fmaf(ml[k].y, c, l);
+#pragma unroll
+            for (int e = 0; e < PER; ++e) acc[e] = fmaf(x[k][e], c, acc[e]);
+        }
+        m = top;
     }
-    if (lane == 0) sum_s[wave] = sum;
+    if (lane == 0) { m_s[team] = m; l_s[team] = l; }
+#pragma unroll
+    for (int e = 0; e < PER; ++e) acc_s[team][lane * PER + e] = acc[e];
     __syncthreads();
     for (int d = threadIdx.x; d < DH; d += 256) {
-        const float s = (sum_s[0] + sum_s[1]) + (sum_s[2] + sum_s[3]);
-        const float a = (acc_s[0][d] + acc_s[1][d]) + (acc_s[2][d] + acc_s[3][d]);
-        p.ctx[b * p.ldo + (long)h * DH + d] = s == 0.0f ? 0.0f : a / s;
+        float top = -INFINITY, sum = 0.0f, a = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) top = fmaxf(top, m_s[k]);
+        const float base = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const float c = __builtin_amdgcn_exp2f(m_s[k] - base);
+            sum = fmaf(l_s[k], c, sum);
+            a = fmaf(acc_s[k][d], c, a);
+        }
+        p.ctx[b * p.ldo + (long)h * DH + d] = sum == 0.0f ? 0.0f : a / sum;
     }
 }
 
-constexpr int SPLIT_MIN_ROWS = 256;                 // rows of the smallest chunk
-
-// How many chunks a call is split into (0: one workgroup per request and key head, one launch)
-int paged_split_target(int B, int H, int kv_heads, int depth, int type, int max_len) {
-    const int n_group = (H / kv_heads + 15) / 16;
-    const long units = (long)B * kv_heads * n_group;
-    if (max_len <= 512) return 0;
-    if (units >= 1024 && max_len <= 2048) return 0;
-    const long per = (long)kv_heads * n_group;
-    const long t = 1024 / per;
-    return (int)(t < 1 ? 1 : t);
+// How many parts a call is cut into (0: one workgroup per request and key head, one launch).
+// Parts: one workgroup per CU.  Its four waves keep 64 KB of keys and values in flight; twice and four times as many workgroups
+// measured the same or less (61 ragged requests up to 4096 rows of bfloat16: 102.2 / 103.0 / 104.5 us with 256 / 512 / 1024; one request of
+// 131071 rows: 97.8 / 98.4 / 101.8).
+// Requests of up to 1024 rows are not cut: the second launch costs what the shorter sweep gains (4 heads of 64, float32, cut / not cut: one
+// request of 600 rows 7.0 / 6.3 us, of 1000 7.0 / 8.0, of 1500 7.0 / 10.1; and a launch less to issue).  Nor are requests of up to 2048
+// where there is a workgroup for every CU anyway (32 heads on 8 of 128, bfloat16, cut / not cut: 32 requests of 2000 51.8 / 49.0 us, 128 185 /
+// 178, but 128 ragged ones 106 / 112).
+int paged_split_target(int B, int H, int kv_heads, int max_len) {
+    const long per = (long)kv_heads * ((H / kv_heads + 15) / 16);
+    if (max_len <= 1024 || (B * per >= 256 && max_len <= 2048)) return 0;
+    return per < 256 ? (int)(256 / per) : 1;
 }
 
 bool bad_cache(const void* k, const void* v, int64_t s_page, int64_t s_head, int64_t s_row, int type, int depth) {
@@ -674,10 +974,16 @@ bool bad_cache(const void* k, const void* v, int64_t s_page, int64_t s_head, int
 
 }  // namespace
 
+constexpr int PLAN_ROWS = 4096;        // rows from which the copies of a plan are a launch of their own
+
+extern "C" int64_t estts_page_plan_ws_bytes(int32_t B, int32_t T) {
+    return B > PLAN_LDS || T > PLAN_ROWS ? 4 * (PLAN_HEAD + 4 * (int64_t)B) : 0;
+}
+
 extern "C" int estts_page_plan(const estts_page_plan_args* args, void* stream) {
     ESTTS_CHECK_ARG(args != nullptr, "estts_page_plan: null args");
     const estts_page_plan_args& a = *args;
-    ESTTS_CHECK_ARG(a.lengths && a.n_new && a.block_table && a.free_pages && a.n_free && a.slots && a.lengths_out && a.n_free_out && a.ws,
+    ESTTS_CHECK_ARG(a.lengths && a.n_new && a.block_table && a.free_pages && a.n_free && a.slots && a.lengths_out && a.n_free_out,
                     "estts_page_plan: null pointer");
     ESTTS_CHECK_ARG(a.B > 0 && a.P > 0 && a.n_pages > 0 && a.T > 0 && a.T < (1 << 30) && a.R >= 0 && a.ld_table >= a.P,
                     "estts_page_plan: bad shape");
@@ -685,7 +991,19 @@ extern "C" int estts_page_plan(const estts_page_plan_args* args, void* stream) {
     ESTTS_CHECK_ARG(a.page > 0 && a.page % 16 == 0, "estts_page_plan: page must be a multiple of 16 (got %d)", a.page);
     ESTTS_CHECK_ARG((int64_t)a.P * a.page < (1LL << 31) && (int64_t)a.n_pages * a.page < (1LL << 31) && (int64_t)a.B * a.P < (1LL << 31),
                     "estts_page_plan: P * page, n_pages * page and B * P must stay below 2^31");
-    ESTTS_LAUNCH(page_plan_kernel, dim3(1), dim3(PLAN_THREADS), 0, (hipStream_t)stream, a);
+    const int64_t need = estts_page_plan_ws_bytes(a.B, a.T);
+    ESTTS_CHECK_ARG(need == 0 || (a.ws && a.ws_bytes >= need), "estts_page_plan: this call needs %ld bytes of scratch (given: %ld)", (long)need, (long)a.ws_bytes);
+    const hipStream_t st = (hipStream_t)stream;
+    const int split = a.T > PLAN_ROWS;
+    if (a.B > PLAN_LDS) ESTTS_LAUNCH((page_plan_kernel<1024, false>), dim3(1), dim3(1024), 0, st, a, split);
+    else if (a.B > 256 || (!split && a.T > 1024)) ESTTS_LAUNCH((page_plan_kernel<1024, true>), dim3(1), dim3(1024), 0, st, a, split);
+    else ESTTS_LAUNCH((page_plan_kernel<256, true>), dim3(1), dim3(256), 0, st, a, split);
+    if (split) {
+        const int wgs = (a.T + 255) / 256;
+        const dim3 grid(wgs < 1024 ? wgs : 1024);
+        if (a.B > PLAN_LDS) ESTTS_LAUNCH(page_copy_kernel<false>, grid, dim3(256), 0, st, a);
+        else ESTTS_LAUNCH(page_copy_kernel<true>, grid, dim3(256), 0, st, a);
+    }
     ESTTS_CHECK_LAUNCH("estts_page_plan");
     return 0;
 }
@@ -714,20 +1032,30 @@ extern "C" int estts_page_write(const estts_page_write_args* args, void* stream)
     return 0;
 }
 
-extern "C" int64_t estts_paged_attention_ws_bytes(int32_t B, int32_t H, int32_t kv_heads, int32_t depth, int32_t type, int32_t max_len) {
+extern "C" int64_t estts_paged_attention_ws_bytes(int32_t B, int32_t H, int32_t kv_heads, int32_t depth, int32_t max_len) {
     if (B <= 0 || H <= 0 || kv_heads <= 0 || H % kv_heads || depth <= 0 || max_len <= 0) return 0;      // (estts_paged_attention says why not)
-    const int target = paged_split_target(B, H, kv_heads, depth, type, max_len);
-    return target ? PagedScratch::bytes((long)target + B, H, depth, B) : 0;
+    const int target = paged_split_target(B, H, kv_heads, max_len);
+    return target ? PagedScratch::bytes(target, H, depth, B) : 0;
 }
 
 template <typename T, int DH>
 static void launch_paged_attention(const estts_paged_attention_args& a, int target, hipStream_t stream) {
-    const int n_items = target ? target + a.B : a.B, n_group = (a.H / a.kv_heads + 15) / 16;
-    const int units = n_items * a.kv_heads;
-    const dim3 grid(n_group > 1 ? (units + 7) / 8 * 8 * n_group : units);
-    if (a.key_mask) ESTTS_LAUNCH((paged_attention_kernel<T, DH, true>), grid, dim3(ATT_WAVES * 64), 0, stream, a, target, SPLIT_MIN_ROWS);
-    else ESTTS_LAUNCH((paged_attention_kernel<T, DH, false>), grid, dim3(ATT_WAVES * 64), 0, stream, a, target, SPLIT_MIN_ROWS);
-    if (target) ESTTS_LAUNCH(paged_join_kernel<DH>, dim3(a.H, a.B), dim3(256), 0, stream, a, n_items);
+    const int group = a.H / a.kv_heads, n_group = (group + 15) / 16;
+    const int units = (target ? target : a.B) * a.kv_heads;
+    const dim3 grid(n_group > 1 ? (units + 7) / 8 * 8 * n_group : units), block(ATT_WAVES * 64);
+    if constexpr (sizeof(T) == 4) {
+        if (group <= FEW_QUERIES) {
+            if (group == 1 && a.key_mask) ESTTS_LAUNCH((paged_attention_few_kernel<DH, true, 1, ATT_WAVES>), grid, block, 0, stream, a, target);
+            else if (group == 1) ESTTS_LAUNCH((paged_attention_few_kernel<DH, false, 1, ATT_WAVES>), grid, block, 0, stream, a, target);
+            else if (a.key_mask) ESTTS_LAUNCH((paged_attention_few_kernel<DH, true, 2, ATT_WAVES>), grid, block, 0, stream, a, target);
+            else ESTTS_LAUNCH((paged_attention_few_kernel<DH, false, 2, ATT_WAVES>), grid, block, 0, stream, a, target);
+            if (target) ESTTS_LAUNCH(paged_join_kernel<DH>, dim3(a.H, a.B), dim3(256), 0, stream, a, target);
+            return;
+        }
+    }
+    if (a.key_mask) ESTTS_LAUNCH((paged_attention_kernel<T, DH, true, ATT_WAVES>), grid, block, 0, stream, a, target);
+    else ESTTS_LAUNCH((paged_attention_kernel<T, DH, false, ATT_WAVES>), grid, block, 0, stream, a, target);
+    if (target) ESTTS_LAUNCH(paged_join_kernel<DH>, dim3(a.H, a.B), dim3(256), 0, stream, a, target);
 }
 
 template <typename T>
@@ -756,10 +1084,10 @@ extern "C" int estts_paged_attention(const estts_paged_attention_args* args, voi
     ESTTS_CHECK_ARG(a.s_row * (int64_t)a.page < (1LL << 28), "estts_paged_attention: the rows of one page must span less than 2^28 elements");
     ESTTS_CHECK_ARG(a.max_len >= 0, "estts_paged_attention: max_len must not be negative");
     if (a.max_len == 0 || (int64_t)a.max_len > (int64_t)a.P * a.page) a.max_len = a.P * a.page;
-    ESTTS_CHECK_ARG((int64_t)a.B * a.max_len < (1LL << 38) && ((int64_t)a.B + 1024) * a.H < (1LL << 28),
-                    "estts_paged_attention: B * max_len must stay below 2^38 and B * H below 2^28");
-    const int target = paged_split_target(a.B, a.H, a.kv_heads, a.depth, a.type, a.max_len);
-    const int64_t need = target ? PagedScratch::bytes((long)target + a.B, a.H, a.depth, a.B) : 0;
+    ESTTS_CHECK_ARG((int64_t)a.B * a.max_len < (1LL << 36) && (int64_t)a.B * a.H < (1LL << 23),
+                    "estts_paged_attention: B * max_len must stay below 2^36 and B * H below 2^23");
+    const int target = paged_split_target(a.B, a.H, a.kv_heads, a.max_len);
+    const int64_t need = target ? PagedScratch::bytes(target, a.H, a.depth, a.B) : 0;
     ESTTS_CHECK_ARG(need == 0 || (a.ws && a.ws_bytes >= need && !(reinterpret_cast<uintptr_t>(a.ws) & 15)),
                     "estts_paged_attention: this call needs %ld bytes of scratch, 16-byte aligned (given: %ld)", (long)need, (long)a.ws_bytes);
     if (a.type == ESTTS_KV_F32) launch_paged_attention<float>(a, target, (hipStream_t)stream);

@@ -156,7 +156,8 @@ class StepProgram:
 
 
 def _stream():
-    return torch.cuda.current_stream().cuda_stream
+    # (the raw handle of torch.cuda.current_stream(), without building the Stream object: 2.7 -> 0.2 us a launch)
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 def _ptr(t):
@@ -631,50 +632,62 @@ def decoder_block_row(wqkv, wos, sa_ln, sa_last_ln, wqc, woc, ca_ln, wff, cache,
 KV_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}     # ESTTS_KV_*
 
 
-def _check_here(what, **tensors):
-    """All tensors on the current device, to whose current stream launches go (None aside)."""
-    for name, t in tensors.items():
-        if t is not None and (not t.is_cuda or t.get_device() != torch.cuda.current_device()):
-            raise ValueError(f'{what}: {name} is on {t.device}, which is not the current device')
+def _check_here(what, names, *tensors):
+    """All tensors on the current device, to whose current stream launches go (None aside).  names: theirs, for the message."""
+    d = tensors[0].get_device()
+    if d < 0 or d != torch._C._cuda_getDevice():
+        i = 0
+    else:
+        for i, t in enumerate(tensors):
+            if t is not None and t.get_device() != d:
+                break
+        else:
+            return
+    raise ValueError(f'{what}: {names.split()[i]} is on {tensors[i].device}, which is not the current device')
 
 
 def _check_rows(what, t, name, rows, width):
-    if t.dtype != torch.float32:
+    """Row stride of a [rows, >= width] float32 view with contiguous rows."""
+    if t.dtype is not torch.float32:
         raise TypeError(f'{what}: {name} must be float32, got {t.dtype}')
-    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] < width or (t.shape[1] > 1 and t.stride(1) != 1):
-        raise ValueError(f'{what}: {name} must be [{rows}, >= {width}] with contiguous rows, got {list(t.shape)} with strides {t.stride()}')
-    return t.stride(0) if rows > 1 else width
+    shape, strides = t.shape, t.stride()
+    if len(shape) != 2 or shape[0] != rows or shape[1] < width or (strides[1] != 1 and shape[1] > 1):
+        raise ValueError(f'{what}: {name} must be [{rows}, >= {width}] with contiguous rows, got {list(shape)} with strides {strides}')
+    return strides[0] if rows > 1 else width
 
 
 def _check_i32(what, t, name, shape):
-    if t.dtype != torch.int32:
+    if t.dtype is not torch.int32:
         raise TypeError(f'{what}: {name} must be int32, got {t.dtype}')
-    if tuple(t.shape) != shape or not t.is_contiguous():
+    if t.shape != shape or not t.is_contiguous():
         raise ValueError(f'{what}: {name} must be a contiguous {list(shape)} tensor, got {list(t.shape)} with strides {t.stride()}')
 
 
-def _check_table(what, block_table, B):
-    if block_table.dtype != torch.int32:
-        raise TypeError(f'{what}: block_table must be int32, got {block_table.dtype}')
-    if block_table.dim() != 2 or block_table.shape[0] != B or block_table.shape[1] < 1 or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
-        raise ValueError(f'{what}: block_table must be [{B}, pages of a request] with contiguous rows, got {list(block_table.shape)}')
-    return block_table.stride(0) if B > 1 else block_table.shape[1]
-
-
-def _page_strides(t):
-    """Element strides of page, head and row of a cache; those of dimensions of size 1, which nothing is multiplied with, as 0 / depth."""
-    n, (p, h, r, _) = t.shape, t.stride()
-    return p if n[0] > 1 else 0, h if n[1] > 1 else 0, r if n[2] > 1 else n[3]
+def _check_table(what, t, B):
+    """(pages of a request, row stride) of a block table [B, P]."""
+    if t.dtype is not torch.int32:
+        raise TypeError(f'{what}: block_table must be int32, got {t.dtype}')
+    shape, strides = t.shape, t.stride()
+    if len(shape) != 2 or shape[0] != B or shape[1] < 1 or (strides[1] != 1 and shape[1] > 1):
+        raise ValueError(f'{what}: block_table must be [{B}, pages of a request] with contiguous rows, got {list(shape)} with strides {strides}')
+    return shape[1], strides[0] if B > 1 else shape[1]
 
 
 def _check_pages(what, k_cache, v_cache):
-    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape or v_cache.dtype != k_cache.dtype or _page_strides(v_cache) != _page_strides(k_cache):
-        raise ValueError(f'{what}: k_cache and v_cache must be [n_pages, kv_heads, page, depth] tensors of the same strides and type')
-    if k_cache.dtype not in KV_TYPES:
-        raise TypeError(f'{what}: caches hold float32, bfloat16 or float16, got {k_cache.dtype}')
-    if k_cache.stride(3) != 1 or v_cache.stride(3) != 1:
-        raise ValueError(f'{what}: the last dimension of the caches must be contiguous')
-    return _page_strides(k_cache)
+    """Shape and strides of a pair of caches [n_pages, kv_heads, page, depth]; the strides of dimensions of size 1, which nothing is
+    multiplied with, as 0 and depth."""
+    n, k, v = k_cache.shape, k_cache.stride(), v_cache.stride()
+    kind = k_cache.dtype
+    if len(n) == 4 and v_cache.shape == n:
+        if 1 in n:
+            k, v = [(s[0] if n[0] > 1 else 0, s[1] if n[1] > 1 else 0, s[2] if n[2] > 1 else n[3], s[3] if n[3] > 1 else 1) for s in (k, v)]
+        if k == v and v_cache.dtype is kind:
+            if kind not in KV_TYPES:
+                raise TypeError(f'{what}: caches hold float32, bfloat16 or float16, got {kind}')
+            if k[3] != 1:
+                raise ValueError(f'{what}: the last dimension of the caches must be contiguous')
+            return n, k
+    raise ValueError(f'{what}: k_cache and v_cache must be [n_pages, kv_heads, page, depth] tensors of the same strides and type')
 
 
 def new_paged_cache(n_pages, page, kv_heads, depth, dtype=torch.float32, device='cuda'):
@@ -690,33 +703,40 @@ def page_plan(lengths, new, block_table, free_pages, n_free, page, slots, positi
     positions: like slots, the place of each row in its request.  lengths and n_free are updated in place unless lengths_out /
     n_free_out are given; refused [1] counts the requests that were turned away (their length stays).  All int32; nothing
     is read back by the host, so a captured step plans itself anew on every replay."""
-    B = lengths.numel()
     lengths_out = lengths if lengths_out is None else lengths_out
     n_free_out = n_free if n_free_out is None else n_free_out
-    for t, n, shape in ((lengths, 'lengths', (B,)), (new, 'new', (B,)), (free_pages, 'free_pages', (free_pages.numel(),)), (n_free, 'n_free', (1,)),
-                        (lengths_out, 'lengths_out', (B,)), (n_free_out, 'n_free_out', (1,)), (slots, 'slots', tuple(slots.shape))):
-        _check_i32('page_plan', t, n, shape)
+    B, T, padded = lengths.numel(), slots.numel(), slots.dim() == 2
+    _check_i32('page_plan', lengths, 'lengths', (B,))
+    _check_i32('page_plan', new, 'new', (B,))
+    _check_i32('page_plan', free_pages, 'free_pages', (free_pages.numel(),))
+    _check_i32('page_plan', n_free, 'n_free', (1,))
+    if lengths_out is not lengths:
+        _check_i32('page_plan', lengths_out, 'lengths_out', (B,))
+    if n_free_out is not n_free:
+        _check_i32('page_plan', n_free_out, 'n_free_out', (1,))
+    _check_i32('page_plan', slots, 'slots', slots.shape)
     if positions is not None:
-        _check_i32('page_plan', positions, 'positions', tuple(slots.shape))
+        _check_i32('page_plan', positions, 'positions', slots.shape)
     if refused is not None:
         _check_i32('page_plan', refused, 'refused', (1,))
-    ld = _check_table('page_plan', block_table, B)
-    if slots.dim() not in (1, 2) or (slots.dim() == 2 and slots.shape[0] != B):
+    P, ld = _check_table('page_plan', block_table, B)
+    if slots.dim() != 1 and not (padded and slots.shape[0] == B):
         raise ValueError(f'page_plan: slots must be [T] (packed rows) or [{B}, R] (padded rows), got {list(slots.shape)}')
-    _check_here('page_plan', lengths=lengths, new=new, block_table=block_table, free_pages=free_pages, n_free=n_free, slots=slots, positions=positions,
-                lengths_out=lengths_out, n_free_out=n_free_out, refused=refused)
-    ws = _scratch(12 * B, lengths.device)
+    _check_here('page_plan', 'lengths new block_table free_pages n_free slots positions lengths_out n_free_out refused', lengths, new, block_table,
+                free_pages, n_free, slots, positions, lengths_out, n_free_out, refused)
+    lib = _lib.load()
+    nbytes = lib.estts_page_plan_ws_bytes(B, T)
+    ws = _scratch(nbytes, lengths.device) if nbytes > 0 else None
     a = _lib.PagePlanArgs(lengths.data_ptr(), new.data_ptr(), block_table.data_ptr(), ld, free_pages.data_ptr(), n_free.data_ptr(), slots.data_ptr(),
-                          _ptr(positions), lengths_out.data_ptr(), n_free_out.data_ptr(), _ptr(refused), ws.data_ptr(),
-                          B, block_table.shape[1], free_pages.numel(), page, slots.numel(), slots.shape[1] if slots.dim() == 2 else 0)
+                          _ptr(positions), lengths_out.data_ptr(), n_free_out.data_ptr(), _ptr(refused), _ptr(ws), nbytes,
+                          B, P, free_pages.numel(), page, T, slots.shape[1] if padded else 0)
     keep = (lengths, new, block_table, free_pages, n_free, slots, positions, lengths_out, n_free_out, refused, ws)
     if _program is not None:
         _program.append(('page_plan', a, keep))
         return slots
-    check(_lib.load().estts_page_plan(a, _stream()), 'estts_page_plan')
+    check(lib.estts_page_plan(a, _stream()), 'estts_page_plan')
     if _trace is not None or _debug_sync:
-        _record('page_plan', {'B': B, 'T': slots.numel(), 'page': page, 'flops': 0.0, 'bytes': 4.0 * (3 * B + 2 * slots.numel())},
-                _lib.load().estts_page_plan, a, keep=keep)
+        _record('page_plan', {'B': B, 'T': T, 'page': page, 'flops': 0.0, 'bytes': 4.0 * (3 * B + 2 * T)}, lib.estts_page_plan, a, keep=keep)
     return slots
 
 
@@ -724,14 +744,13 @@ def page_write(k, v, k_cache, v_cache, slots):
     """Rows k, v ([T, >= kv_heads * depth] float32 views, head after head) into the pages (estts_page_write): row t goes to slots[t]
     (int32, any shape with T elements; page * page size + row, what page_plan writes), rounded to the caches' type; rows with a
     slot outside the cache go nowhere.  The slots of a call must be distinct."""
-    s_page, s_head, s_row = _check_pages('page_write', k_cache, v_cache)
-    n_pages, Hk, page, D = k_cache.shape
+    (n_pages, Hk, page, D), (s_page, s_head, s_row, _) = _check_pages('page_write', k_cache, v_cache)
     if (n_pages > 1 and not s_page) or (Hk > 1 and not s_head) or not s_row:
         raise ValueError('page_write: the caches must not be broadcast views')
     T = slots.numel()
-    _check_i32('page_write', slots, 'slots', tuple(slots.shape))
+    _check_i32('page_write', slots, 'slots', slots.shape)
     ldk, ldv = _check_rows('page_write', k, 'k', T, Hk * D), _check_rows('page_write', v, 'v', T, Hk * D)
-    _check_here('page_write', k=k, v=v, k_cache=k_cache, v_cache=v_cache, slots=slots)
+    _check_here('page_write', 'k v k_cache v_cache slots', k, v, k_cache, v_cache, slots)
     a = _lib.PageWriteArgs(k.data_ptr(), ldk, v.data_ptr(), ldv, k_cache.data_ptr(), v_cache.data_ptr(), s_page, s_head, s_row, slots.data_ptr(),
                            T, Hk, D, page, n_pages, KV_TYPES[k_cache.dtype])
     keep = (k, v, k_cache, v_cache, slots)
@@ -752,11 +771,9 @@ def paged_attention(q, k_cache, v_cache, block_table, lengths, ctx, heads, key_m
     left out; a request with nothing left gets zeros.  scale: 1 / sqrt(depth) if None.  max_len: bound on the lengths that the host
     knows of (P * page if None; rows past it are not read)."""
     B = lengths.numel()
-    s_page, s_head, s_row = _check_pages('paged_attention', k_cache, v_cache)
+    (n_pages, Hk, page, D), (s_page, s_head, s_row, _) = _check_pages('paged_attention', k_cache, v_cache)
     _check_i32('paged_attention', lengths, 'lengths', (B,))
-    ld = _check_table('paged_attention', block_table, B)
-    n_pages, Hk, page, D = k_cache.shape
-    P = block_table.shape[1]
+    P, ld = _check_table('paged_attention', block_table, B)
     max_len = P * page if max_len is None else min(int(max_len), P * page)
     if max_len < 1:
         raise ValueError('paged_attention: max_len must be positive')
@@ -771,9 +788,9 @@ def paged_attention(q, k_cache, v_cache, block_table, lengths, ctx, heads, key_m
         if key_mask.dim() != 2 or key_mask.shape[0] != B or key_mask.shape[1] < max_len:
             raise ValueError(f'paged_attention: key_mask must be [{B}, >= {max_len}], got {list(key_mask.shape)}')
         sb, ss = key_mask.stride()
-    _check_here('paged_attention', q=q, k_cache=k_cache, v_cache=v_cache, block_table=block_table, lengths=lengths, ctx=ctx, key_mask=key_mask)
+    _check_here('paged_attention', 'q k_cache v_cache block_table lengths ctx key_mask', q, k_cache, v_cache, block_table, lengths, ctx, key_mask)
     lib, kind = _lib.load(), KV_TYPES[k_cache.dtype]
-    nbytes = lib.estts_paged_attention_ws_bytes(B, heads, Hk, D, kind, max_len)
+    nbytes = lib.estts_paged_attention_ws_bytes(B, heads, Hk, D, max_len)
     ws = _scratch(nbytes, q.device) if nbytes > 0 else None
     a = _lib.PagedAttentionArgs(q.data_ptr(), ldq, k_cache.data_ptr(), v_cache.data_ptr(), s_page, s_head, s_row,
                                 block_table.data_ptr(), ld, lengths.data_ptr(), _ptr(key_mask), sb, ss, ctx.data_ptr(),

@@ -912,18 +912,20 @@ int estts_prenet_row(const estts_prenet_row_args* args, void* stream);
  *   lengths_out[b] = 0 (ended), lengths[b] + n_new[b] (granted) or lengths[b] (refused);  n_free_out[0] = height of the stack now;
  *   refused[0] = number of requests that asked and were not granted (may be NULL)
  * lengths_out may be lengths and n_free_out may be n_free (the state of a decoding loop); block_table and free_pages are updated in
- * place, and only where the rules above write.  ws: 3 B int32 of scratch that belong to this call until it has run. */
+ * place, and only where the rules above write.  ws: estts_page_plan_ws_bytes() bytes (may be NULL where that is 0) that belong to this
+ * call until it has run. */
 typedef struct estts_page_plan_args {
     const int32_t* lengths; const int32_t* n_new;
     int32_t* block_table; int64_t ld_table;
     int32_t* free_pages; const int32_t* n_free;
     int32_t* slots; int32_t* positions;
     int32_t* lengths_out; int32_t* n_free_out; int32_t* refused;
-    int32_t* ws;
+    int32_t* ws; int64_t ws_bytes;
     int32_t B, P, n_pages, page, T, R;
 } estts_page_plan_args;
 
 int estts_page_plan(const estts_page_plan_args* args, void* stream);
+int64_t estts_page_plan_ws_bytes(int32_t B, int32_t T);
 
 /* K / V rows into the pages: for t < T with 0 <= slots[t] < n_pages page, rows k[t], v[t] (float32, head h at columns [h depth, (h + 1) depth))
  * go to that slot, rounded to the cache's type (to nearest, ties to even); everything else stays as it was.  The slots of one call
@@ -960,7 +962,7 @@ typedef struct estts_paged_attention_args {
 } estts_paged_attention_args;
 
 int estts_paged_attention(const estts_paged_attention_args* args, void* stream);
-int64_t estts_paged_attention_ws_bytes(int32_t B, int32_t H, int32_t kv_heads, int32_t depth, int32_t type, int32_t max_len);
+int64_t estts_paged_attention_ws_bytes(int32_t B, int32_t H, int32_t kv_heads, int32_t depth, int32_t max_len);
 
 /* ------------------------------------------------------------------------------------------
  * Step programs: a fixed sequence of launches whose arguments depend affinely on a step index (an incremental decoder:

@@ -35,7 +35,7 @@ def test_field_offsets_match_header_layout(tmp_path, cname):
 # ---------------------------------------------------------------------------------------------------------------- C ABI refusals
 def plan_block(**kw):
     f = dict(lengths=FAKE, n_new=FAKE, block_table=FAKE, ld_table=8, free_pages=FAKE, n_free=FAKE, slots=FAKE, positions=FAKE, lengths_out=FAKE,
-             n_free_out=FAKE, refused=FAKE, ws=FAKE, B=4, P=8, n_pages=32, page=16, T=4, R=1)
+             n_free_out=FAKE, refused=FAKE, B=4, P=8, n_pages=32, page=16, T=4, R=1)
     f.update(kw)
     return _lib.PagePlanArgs(**f)
 
@@ -54,8 +54,9 @@ def attention_block(**kw):
     return _lib.PagedAttentionArgs(**f)
 
 
-@pytest.mark.parametrize('bad,word', [(dict(lengths=None), 'null'), (dict(ws=None), 'null'), (dict(B=0), 'shape'), (dict(T=0), 'shape'),
-                                      (dict(ld_table=7), 'shape'), (dict(R=2), 'padded'), (dict(page=8), 'multiple of 16'), (dict(page=0), 'multiple of 16'),
+@pytest.mark.parametrize('bad,word', [(dict(lengths=None), 'null'), (dict(free_pages=None), 'null'), (dict(B=0), 'shape'), (dict(T=0), 'shape'),
+                                      (dict(ld_table=7), 'shape'), (dict(R=2), 'padded'), (dict(T=5000, R=0), 'scratch'),
+                                      (dict(T=5000, R=0, ws=FAKE, ws_bytes=79), 'scratch'), (dict(B=5000, T=5000), 'scratch'), (dict(page=8), 'multiple of 16'), (dict(page=0), 'multiple of 16'),
                                       (dict(page=24), 'multiple of 16'), (dict(n_pages=1 << 27), '2^31'), (dict(P=1 << 27, ld_table=1 << 27), '2^31')])
 def test_page_plan_refuses(bad, word):
     lib = _lib.load()
