@@ -237,20 +237,28 @@ template <> struct Kv16<_Float16> {
     static __device__ __forceinline__ f32x4 mfma(Frag a, Frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 };
 
-// x = sum of the pieces up to 2^-24 (bfloat16) or 2^-22 (float16) of x
+// x = sum of the pieces up to 2^-24 (bfloat16) or 2^-22 (float16) of x; two values to a conversion
 template <typename T>
 __device__ __forceinline__ void split_pieces(const float (&x)[8], typename Kv16<T>::Frag (&f)[Kv16<T>::PIECES]) {
-    float r[8];
+    typedef __attribute__((ext_vector_type(2))) T pair_t;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) r[e] = x[e];
+    for (int e = 0; e < 8; e += 2) {
+        f32x2_t r = {x[e], x[e + 1]};
 #pragma unroll
-    for (int n = 0; n < Kv16<T>::PIECES; ++n)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const T h = (T)r[e];
-            f[n][e] = h;
-            r[e] -= (float)h;
+        for (int n = 0; n < Kv16<T>::PIECES; ++n) {
+            const pair_t h = __builtin_convertvector(r, pair_t);
+            f[n][e] = h[0];
+            f[n][e + 1] = h[1];
+            if (n + 1 < Kv16<T>::PIECES) r -= __builtin_convertvector(h, f32x2_t);
         }
+    }
+}
+
+// 16 bytes (8, 4) at byte `lane_at` + `at` behind a base that is the same for the whole wave: the base and `at` stay in scalar registers
+typedef __attribute__((ext_vector_type(4))) int i32x4;
+typedef __attribute__((ext_vector_type(2))) int i32x2;
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t wave_rows(const char* base, int bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, bytes, 0x00027000);
 }
 
 __device__ __forceinline__ int request_rows(const estts_paged_attention_args& p, int b) {
@@ -501,17 +509,18 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_attention_kernel(const estts
         // registers of a tile
         constexpr int KL = F32 ? DH / 16 : DH / 32;         // 16-byte loads of K per half and lane
         constexpr int VW = NV * (int)sizeof(T) / 4;         // dwords of V per row and lane
-        int4 kr[HALVES][KL];
+        i32x4 kr[HALVES][KL];
         int vr[HALVES][4][VW];
         [[maybe_unused]] float mk[HALVES][4];
         const int k_lane = i * row_bytes + 16 * g;
         const int v_lane = 4 * g * row_bytes + i * NV * (int)sizeof(T);
+        const int half_bytes = 15 * row_bytes + DH * (int)sizeof(T);
         auto load_k = [&](int it) {
 #pragma unroll
             for (int s = 0; s < HALVES; ++s) {
-                const char* at = kbase + walk.at[s];
+                const auto rows = wave_rows(kbase + walk.at[s], half_bytes);
 #pragma unroll
-                for (int x = 0; x < KL; ++x) kr[s][x] = *reinterpret_cast<const int4*>(at + (unsigned)(k_lane + 64 * x));
+                for (int x = 0; x < KL; ++x) kr[s][x] = __builtin_amdgcn_raw_buffer_load_b128(rows, k_lane + 64 * x, 0, 0);
             }
             if constexpr (MASK) {
                 const float* mrow = p.key_mask + b * p.mask_sb;
@@ -525,21 +534,20 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_attention_kernel(const estts
         auto load_v = [&]() {
 #pragma unroll
             for (int s = 0; s < HALVES; ++s) {
-                const char* at = vbase + walk.at[s];
+                const auto rows = wave_rows(vbase + walk.at[s], half_bytes);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const char* a = at + (unsigned)(v_lane + j * row_bytes);
                     if constexpr (VW >= 4) {
 #pragma unroll
                         for (int x = 0; x < VW / 4; ++x) {
-                            const int4 t = *reinterpret_cast<const int4*>(a + 16 * x);
+                            const i32x4 t = __builtin_amdgcn_raw_buffer_load_b128(rows, v_lane + 16 * x, j * row_bytes, 0);
                             vr[s][j][4 * x] = t.x; vr[s][j][4 * x + 1] = t.y; vr[s][j][4 * x + 2] = t.z; vr[s][j][4 * x + 3] = t.w;
                         }
                     } else if constexpr (VW == 2) {
-                        const int2 t = *reinterpret_cast<const int2*>(a);
+                        const i32x2 t = __builtin_amdgcn_raw_buffer_load_b64(rows, v_lane, j * row_bytes, 0);
                         vr[s][j][0] = t.x; vr[s][j][VW - 1] = t.y;
                     } else {
-                        vr[s][j][0] = *reinterpret_cast<const int*>(a);
+                        vr[s][j][0] = __builtin_amdgcn_raw_buffer_load_b32(rows, v_lane, j * row_bytes, 0);
                     }
                 }
             }
@@ -568,10 +576,11 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_attention_kernel(const estts
                         f32x4 a0 = {0.0f, 0.0f, 0.0f, 0.0f}, a1 = a0;
 #pragma unroll
                         for (int x = 0; x < KL; ++x) {
-                            a0 = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, kr[s][x].x), qx[4 * x], a0, 0, 0, 0);
-                            a1 = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, kr[s][x].y), qx[4 * x + 1], a1, 0, 0, 0);
-                            a0 = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, kr[s][x].z), qx[4 * x + 2], a0, 0, 0, 0);
-                            a1 = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, kr[s][x].w), qx[4 * x + 3], a1, 0, 0, 0);
+                            const f32x4 kf = __builtin_bit_cast(f32x4, kr[s][x]);
+                            a0 = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[0], qx[4 * x], a0, 0, 0, 0);
+                            a1 = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[1], qx[4 * x + 1], a1, 0, 0, 0);
+                            a0 = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[2], qx[4 * x + 2], a0, 0, 0, 0);
+                            a1 = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[3], qx[4 * x + 3], a1, 0, 0, 0);
                         }
 #pragma unroll
                         for (int j = 0; j < 4; ++j) sc[s][j] = a0[j] + a1[j];
@@ -603,16 +612,18 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_attention_kernel(const estts
                 bool all_in = r0 + TILE <= end;
 #pragma unroll
                 for (int s = 0; s < HALVES; ++s) all_in = all_in && ok_now[s];
-                bool in[HALVES][4];
+                bool in[HALVES][4], drop = !all_in;
+                auto find_in = [&]() {
 #pragma unroll
-                for (int s = 0; s < HALVES; ++s)
+                    for (int s = 0; s < HALVES; ++s)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        in[s][j] = ok_now[s] && r0 + 16 * s + 4 * g + j < end;
-                        if constexpr (MASK) in[s][j] = in[s][j] && mk[s][j] == 0.0f;
-                    }
-                bool drop = !all_in;
+                        for (int j = 0; j < 4; ++j) {
+                            in[s][j] = ok_now[s] && r0 + 16 * s + 4 * g + j < end;
+                            if constexpr (MASK) in[s][j] = in[s][j] && mk[s][j] == 0.0f;
+                        }
+                };
                 if constexpr (MASK) {
+                    find_in();
                     bool mine = true;
 #pragma unroll
                     for (int s = 0; s < HALVES; ++s)
@@ -626,6 +637,7 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_attention_kernel(const estts
                 walk.locate(nx, nx != it);
                 load_k(nx);
                 if (drop) {
+                    if constexpr (!MASK) find_in();
 #pragma unroll
                     for (int s = 0; s < HALVES; ++s)
 #pragma unroll
