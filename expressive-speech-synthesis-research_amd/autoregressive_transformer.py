@@ -548,6 +548,151 @@ class AutoregressiveTransformer:
         return {'mel': final[:steps * r].clone(), 'decoder_attention': dec_attn, 'text_encoder_attention': text_attn,
                 'gst_encoder_attention': gst_attn, 'gst_tokens': gst_tokens}
 
+    def predict_many(self, inputs, targets=None, spk_embeds=None, max_length=1000, encode=True, stop_check_every=8, cache_dtype=torch.float32,
+                     program=True, dropout_seed=None):
+        """predict() for a list of utterances that decode side by side, one position of each per step (no counterpart in the
+        reference, whose loop runs one utterance at a time: AutoregressiveTransformer.py:279-296).  inputs: phoneme strings or token
+        id sequences of any lengths; targets: list of reference mels or None; spk_embeds: list of speaker embeddings or None.  Returns
+        a list of predict()-style dicts in input order.
+
+        The decoder's self-attention keeps its keys and values in pages (ops.page_plan / page_write / paged_attention): every step
+        plans on the GPU where each utterance's new row goes, an utterance that has stopped gives its pages back and its row attends
+        nothing from then on.  cache_dtype: type of the pages (float32 gives predict()'s numbers up to summation order; bfloat16 or
+        float16 halve what a step reads).  As in predict(), stop decisions are read back once per stop_check_every steps and what an
+        utterance decoded past its stop is dropped.  With decoder_prenet_dropout > 0 the masks are those of generator row
+        step * utterances + utterance."""
+        dev, f32, i32 = self.device, dict(dtype=torch.float32, device=self.device), dict(dtype=torch.int32, device=self.device)
+        M = len(inputs)
+        for name, given in (('targets', targets), ('spk_embeds', spk_embeds)):
+            if given is not None and len(given) != M:
+                raise ValueError(f'predict_many: {M} inputs but {len(given)} {name}')
+        if M == 0:
+            return []
+        rate = self.decoder_prenet_dropout
+        seed = self._next_dropout_seed() if dropout_seed is None else int(dropout_seed) & 0xFFFFFFFF
+        pr = ops.precision_at(self.precision, 'incremental')
+        d, r, C = self.dd, self.r, self.mel_channels
+        blocks = self.decoder.blocks
+        if any(d // sa.heads not in (32, 64, 128) for sa, _, _ in blocks):
+            raise ValueError('predict_many: paged attention takes heads of depth 32, 64 or 128')
+        if not bool((self.start_vec != 0).any()):
+            raise ValueError('predict_many: the start vector must not be all zeros (its position would be masked and nothing left to attend)')
+        S = int(max_length // r) + 1                                  # decoder steps at most
+        if (S - 1) * r >= self.pe_dec.shape[0]:
+            raise ValueError('max_length exceeds decoder_max_position_encoding')
+        encoded = []
+        for m, inp in enumerate(inputs):
+            tokens = torch.as_tensor(np.asarray(self.encode_text(inp) if encode else inp), dtype=torch.int32, device=dev)[None]
+            spk = None if spk_embeds is None else torch.as_tensor(spk_embeds[m], dtype=torch.float32, device=dev)[None]
+            encoded.append(self.call_encoder(tokens, None if targets is None else self.encode_ref(targets[m]), spk))
+        # encoder rows of all utterances, padded with zero rows (which row_zero_mask masks), keys / values once per block
+        lengths_enc = [e[0].shape[1] for e in encoded]
+        N = -(-max(lengths_enc) // 4) * 4
+        enc = torch.zeros(M, N, self.enc_dim, **f32)
+        for m, e in enumerate(encoded):
+            enc[m, :lengths_enc[m]].copy_(e[0][0])
+        enc2, enc_mask = enc.view(M * N, -1), torch.empty(M, N, **f32)
+        ops.row_zero_mask(enc2, enc_mask.view(-1))
+        kv_enc = [torch.empty(M * N, 2 * d, **f32) for _ in blocks]
+        for (_, ca, _), kv in zip(blocks, kv_enc):
+            ca.project_kv(enc2, kv, pr)
+        attn = [torch.empty(S, M, ca.heads, 1, N, **f32) for _, ca, _ in blocks]
+        # pages of the self-attention: one plan for all blocks, a pair of caches for each
+        page = 16
+        P = -(-S // page)
+        caches = [ops.new_paged_cache(M * P, page, sa.heads, d // sa.heads, dtype=cache_dtype, device=dev) for sa, _, _ in blocks]
+        lengths, new = torch.zeros(M, **i32), torch.ones(M, **i32)
+        table, slots = torch.zeros(M, P, **i32), torch.empty(M, 1, **i32)
+        free, n_free = torch.arange(M * P, **i32), torch.full((1,), M * P, **i32)
+        # histories of the causal convolutions: per utterance, `lead` zero rows in front
+        conv_hist, conv_dense = [], []
+        for _, _, ff in blocks:
+            layers = [] if isinstance(ff, FFNLayer) else ff.layers
+            conv_hist.append([torch.zeros(M, layers[0].taps - 1 + S, lin.c_per_tap, **f32) for lin in layers])
+            conv_dense.append([self._as_dense(lin) for lin in layers])
+        kp = self.postnet.layers[0].taps
+        lead = max(kp - 1, r)                                         # (frames and mel rows with the same pitch)
+        post_hist = [torch.zeros(M, lead + S * r, lin.c_per_tap, **f32) for lin in self.postnet.layers]
+        post_dense = [self._as_dense(lin) for lin in self.postnet.layers]
+        # row lead - 1 + i r of `frames` feeds step i: the start vector, then the last frame of every earlier step
+        frames = torch.zeros(M, lead + S * r, C, **f32)
+        frames[:, lead - 1].copy_(self.start_vec.expand(M, C))
+        stop = torch.empty(M, S * r, 3, **f32)
+        dec_mask = torch.zeros(S, M, **f32)
+        xc, xc2, qkv = torch.empty(M, 2 * d, **f32), torch.empty(M, 2 * d, **f32), torch.empty(M, 3 * d, **f32)
+        y, x2, q = torch.empty(M, d, **f32), torch.empty(M, d, **f32), torch.empty(M, d, **f32)
+        p1, hid = torch.empty(M, self.prenet1.N, **f32), torch.empty(M, max(self.decoder.hidden, 4), **f32)
+        lin_r = self._final_proj(r)
+        sqrt_d = math.sqrt(np.float32(d))
+
+        def each(lin, src, src_pitch, dst, residual=None):
+            """The r rows src of utterance 0 through lin to dst, and those of the others at the buffers' pitches."""
+            ops.gemm(src, lin, dst[0], residual=None if residual is None else residual[0], precision=pr, batch=(M, src_pitch, 0, dst.stride(0), 0))
+
+        def step(i):
+            frame = frames[:, lead - 1 + i * r]
+            ops.row_zero_mask(frame, dec_mask[i])
+            ops.gemm(frame, self.prenet1, p1, precision=pr, dropout=(rate, seed, 0, i * M))
+            ops.gemm(p1, self.prenet2, xc[:, :d], alpha=sqrt_d, residual=self.pe_dec[i * r:i * r + 1], r_mod=1, precision=pr,
+                     dropout=(rate, seed, 1, i * M))
+            ops.page_plan(lengths, new, table, free, n_free, page, slots)
+            for b, (sa, ca, ff) in enumerate(blocks):
+                ops.gemm(xc[:, :d], sa.qkv, qkv, precision=pr)
+                ops.page_write(qkv[:, d:2 * d], qkv[:, 2 * d:], *caches[b], slots)
+                ops.paged_attention(qkv[:, :d], *caches[b], table, lengths, xc[:, d:], sa.heads, key_mask=dec_mask.t(), max_len=S)
+                ops.gemm(xc, sa.out, y, precision=pr)
+                ops.rownorm(y, xc2[:, :d], ln_a=sa.ln, residual=xc[:, :d], ln_b=sa.last_ln)
+                ops.gemm(xc2[:, :d], ca.wq, q, precision=pr)
+                ops.attention(q, kv_enc[b][:, :d], kv_enc[b][:, d:], xc2[:, d:], M, ca.heads, 1, N, d // ca.heads, key_mask=enc_mask,
+                              attn=attn[b][i], precision=pr)
+                ops.gemm(xc2, ca.out, y, precision=pr)
+                if isinstance(ff, FFNLayer):
+                    ops.rownorm(y, x2, residual=xc2[:, :d], ln_b=ca.ln)
+                    ff.run(x2, hid, y, xc[:, :d], pr)
+                else:
+                    hist, dense = conv_hist[b], conv_dense[b]
+                    k = ff.layers[0].taps
+                    src = hist[0][:, k - 1 + i]                        # this position's row of the first history
+                    ops.rownorm(y, src, residual=xc2[:, :d], ln_b=ca.ln)
+                    for li, lin in enumerate(dense):
+                        last = li == len(dense) - 1
+                        ops.gemm(hist[li][:, i:i + k].flatten(1), lin, xc[:, :d] if last else hist[li + 1][:, k - 1 + i],
+                                 residual=src if last else None, precision=pr)
+            t0, t1 = lead + i * r, lead + (i + 1) * r
+            mel = post_hist[0][:, t0:t1]                               # FinalProj writes the r new mel frames here
+            ops.gemm(xc[:, :d], lin_r, mel.flatten(1), precision=pr)
+            each(self.stop_linear, mel[0], mel.stride(0), stop[:, i * r:(i + 1) * r])
+            for li, lin in enumerate(post_dense):
+                last = li == len(post_dense) - 1
+                h = post_hist[li]
+                each(lin, self._windows(h[0], t0 - kp + 1, r, kp, lin.K // kp), h.stride(0), frames[:, t0:t1] if last else post_hist[li + 1][:, t0:t1],
+                     residual=mel if last else None)
+
+        prog = ops.StepProgram(step) if program and S >= 2 else None
+        group = max(1, int(stop_check_every))
+        steps, i = [0] * M, 0
+        while i < S and 0 in steps:
+            n = min(group, S - i)
+            for j in range(i, i + n):
+                if prog is not None:
+                    prog.run(j)
+                else:
+                    step(j)
+            rows = stop[:, (i + 1) * r - 1:(i + n) * r:r].cpu()        # the last frame's stop logits of every step of the group
+            ended = (torch.argmax(rows, dim=-1) == self.stop_prob_index).tolist()
+            for m in range(M):
+                if steps[m] == 0 and any(ended[m]):
+                    steps[m] = i + ended[m].index(True) + 1
+            i += n
+            new.copy_(torch.tensor([-1 if s else 1 for s in steps], dtype=torch.int32))
+        results = []
+        for m, (_, _, text_attn, gst_attn, gst_tokens, _, _) in enumerate(encoded):
+            T = steps[m] or S
+            dec_attn = {name: a[:T, m, :, 0, :lengths_enc[m]].permute(1, 0, 2)[None].contiguous() for name, a in zip(self.decoder.names, attn)}
+            results.append({'mel': frames[m, lead:lead + T * r].clone(), 'decoder_attention': dec_attn, 'text_encoder_attention': text_attn,
+                            'gst_encoder_attention': gst_attn, 'gst_tokens': gst_tokens})
+        return results
+
     def predict(self, inp, targets, spk_embed, max_length=1000, encode=True, verbose=True, kv_cache=True, stop_check_every=8):
         """AutoregressiveTransformer.py:265-296.  inp: phoneme string (encode=True) or token ids; targets: reference mel
         (T, 80) for the style encoder or None; spk_embed: (1, D) or None.
