@@ -207,8 +207,8 @@ __global__ __launch_bounds__(256) void page_write_kernel(const estts_page_write_
 //
 // A wave sweeps tiles of 16 (float32, depth 128) or 32 rows for up to 16 query heads that share a key head, on the matrix cores:
 //   S^T (16 rows x 16 queries) = K Q^T      A = K: lane (i, g) holds row i, elements 8g .. 8g+7 of a step of 32 (float32: 4g .. 4g+3 of 16)
-//   O^T (16 features x 16 queries) += V^T P^T   A = V^T: row r of the result is feature r * depth/16 + e in tile e, so that lane i loads the
-//       depth/16 consecutive features of a row that it feeds to all tiles, and a row of V is one coalesced load of 16 lanes
+//   O^T (16 features x 16 queries) += V^T P^T   A = V^T: row r of the result is feature r * depth/16 + e in tile e (feature_of), so that lane i
+//       loads consecutive features of a row for several tiles, and every load of 16 lanes takes whole lines of V
 // The result layout D[4g + j][i] puts the weights of rows 4g + j into lane (i, g), which is where the second product wants them: of
 // two 16-row halves (16-bit types: k slot 8g + 4 half + j is row 16 half + 4g + j) or as they are (float32: k slot g).  Nothing crosses
 // lanes but the maximum.  16-bit values of V are interleaved from rows to features with one v_perm_b32 per two values.
@@ -224,6 +224,18 @@ constexpr int FEW_QUERIES = 2;         // query heads per key head up to which f
 
 // 16-row halves of a wave's tile
 constexpr int tile_halves(int depth, int esize) { return depth * esize == 512 ? 1 : 2; }
+
+// which feature lane (matrix row) r holds as its e-th: consecutive ones, 16 bytes of them at a time over the 16 lanes
+template <int DH, int ESIZE>
+__host__ __device__ constexpr int feature_of(int r, int e) {
+    constexpr int NV = DH / 16, RUN = NV * ESIZE < 16 ? NV : 16 / ESIZE;
+    return (e / RUN) * (16 * RUN) + r * RUN + e % RUN;
+}
+
+// Cache policy of the loads of V (the nt bit): not kept in the caches on the way.  Where the rows are more than the caches hold from one
+// call to the next this reads faster, where they are not it costs what they would have held (see stream_rows).  Not for K, whose
+// lines are read by two instructions.
+constexpr int LOAD_STREAM = 2;
 
 template <typename T> struct Kv16 { typedef bf16x8 Frag; static constexpr int PIECES = 1; };      // (float32: not used)
 template <> struct Kv16<__bf16> {
@@ -436,12 +448,13 @@ __device__ __forceinline__ void join_waves(const estts_paged_attention_args& p, 
     }
 }
 
-template <typename T, int DH, bool MASK, int NW>
+template <typename T, int DH, bool MASK, bool STREAM, int NW>
 __global__ __launch_bounds__(NW * 64, 2) void paged_attention_kernel(const estts_paged_attention_args p, const int target) {
     constexpr bool F32 = sizeof(T) == 4;
     constexpr int HALVES = tile_halves(DH, sizeof(T));
     constexpr int TILE = 16 * HALVES;
-    constexpr int NV = DH / 16;                         // consecutive features of a row of V per lane = tiles of 16 features
+    constexpr int NV = DH / 16;                         // features of a row of V per lane = tiles of 16 features
+    constexpr int VB = NV * (int)sizeof(T) < 16 ? NV * (int)sizeof(T) : 16;     // bytes of one load of them
     __shared__ __attribute__((aligned(16))) float o_s[NW][16][DH];
     __shared__ float m_s[NW][16], l_s[NW][16];
 
@@ -513,7 +526,7 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_attention_kernel(const estts
         int vr[HALVES][4][VW];
         [[maybe_unused]] float mk[HALVES][4];
         const int k_lane = i * row_bytes + 16 * g;
-        const int v_lane = 4 * g * row_bytes + i * NV * (int)sizeof(T);
+        const int v_lane = 4 * g * row_bytes + i * VB;
         const int half_bytes = 15 * row_bytes + DH * (int)sizeof(T);
         auto load_k = [&](int it) {
 #pragma unroll
@@ -531,6 +544,7 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_attention_kernel(const estts
                     for (int j = 0; j < 4; ++j) mk[s][j] = mrow[min(r0 + 16 * s + j, end - 1) * p.mask_ss];
             }
         };
+        constexpr int POLICY = STREAM ? LOAD_STREAM : 0;
         auto load_v = [&]() {
 #pragma unroll
             for (int s = 0; s < HALVES; ++s) {
@@ -540,14 +554,14 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_attention_kernel(const estts
                     if constexpr (VW >= 4) {
 #pragma unroll
                         for (int x = 0; x < VW / 4; ++x) {
-                            const i32x4 t = __builtin_amdgcn_raw_buffer_load_b128(rows, v_lane + 16 * x, j * row_bytes, 0);
-                            vr[s][j][4 * x] = t.x; vr[s][j][4 * x + 1] = t.y; vr[s][j][4 * x + 2] = t.z; vr[s][j][4 * x + 3] = t.w;
+                            const i32x4 t = __builtin_amdgcn_raw_buffer_load_b128(rows, v_lane + 256 * x, j * row_bytes, POLICY);
+                            vr[s][j][4 * x] = t[0]; vr[s][j][4 * x + 1] = t[1]; vr[s][j][4 * x + 2] = t[2]; vr[s][j][4 * x + 3] = t[3];
                         }
                     } else if constexpr (VW == 2) {
-                        const i32x2 t = __builtin_amdgcn_raw_buffer_load_b64(rows, v_lane, j * row_bytes, 0);
-                        vr[s][j][0] = t.x; vr[s][j][VW - 1] = t.y;
+                        const i32x2 t = __builtin_amdgcn_raw_buffer_load_b64(rows, v_lane, j * row_bytes, POLICY);
+                        vr[s][j][0] = t[0]; vr[s][j][VW - 1] = t[1];
                     } else {
-                        vr[s][j][0] = __builtin_amdgcn_raw_buffer_load_b32(rows, v_lane, j * row_bytes, 0);
+                        vr[s][j][0] = __builtin_amdgcn_raw_buffer_load_b32(rows, v_lane, j * row_bytes, POLICY);
                     }
                 }
             }
@@ -711,7 +725,7 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_attention_kernel(const estts
             for (int j = 0; j < 4; ++j)
 #pragma unroll
                 for (int e = 0; e < NV; e += NV < 4 ? NV : 4) {
-                    float* at = &o_s[wave][i][(4 * g + j) * NV + e];
+                    float* at = &o_s[wave][i][feature_of<DH, sizeof(T)>(4 * g + j, e)];
                     if constexpr (NV >= 4) *reinterpret_cast<float4*>(at) = make_float4(o[e][j], o[e + 1][j], o[e + 2][j], o[e + 3][j]);
                     else *reinterpret_cast<float2*>(at) = make_float2(o[e][j], o[e + 1][j]);
                 }
@@ -725,7 +739,7 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_attention_kernel(const estts
 // The same for float32 pages and a key head that only one or two query heads read (NQ): most columns of a matrix tile would be empty
 // and its 64 float32 matrix instructions a tile (2048 cycles) would set the time of a short request.  On the vector ALU a tile
 // is 64 multiply-adds, 32 data-parallel additions and 8 exponentials a lane and query (some 700 cycles).  Lane (i, g) holds the
-// depth/16 features from i depth/16 on of rows 4g + j of a half, of K as of V; the sixteen lanes of a row add up its score.
+// depth/16 features of rows 4g + j of a half that feature_of says, of K as of V; the sixteen lanes of a row add up its score.
 // One request of 1000 rows, 4 key heads of 64 / 128, matrix cores / here: one query head each 13.4 / 8.0 and 22.2 / 10.7 us, two 13.6 / 10.6
 // and 22.4 / 14.8; 64 such requests, bound by memory: 26.5 / 25.4 and 48.3 / 47.2 us (5.3 and 5.7 TB/s).
 __device__ __forceinline__ float row_sum(float v) {     // over the 16 lanes of a row, to all of them
@@ -738,9 +752,10 @@ __device__ __forceinline__ float row_sum(float v) {     // over the 16 lanes of 
     return v;
 }
 
-template <int DH, bool MASK, int NQ, int NW>
+template <int DH, bool MASK, bool STREAM, int NQ, int NW>
 __global__ __launch_bounds__(NW * 64, 2) void paged_attention_few_kernel(const estts_paged_attention_args p, const int target) {
-    constexpr int HALVES = tile_halves(DH, 4), TILE = 16 * HALVES, NV = DH / 16;
+    constexpr int HALVES = tile_halves(DH, 4), TILE = 16 * HALVES, NV = DH / 16, RUN = NV < 4 ? NV : 4;
+    typedef __attribute__((ext_vector_type(RUN))) float run_t;
     __shared__ __attribute__((aligned(16))) float o_s[NW][NQ][DH];
     __shared__ float m_s[NW][NQ], l_s[NW][NQ];
     const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
@@ -758,34 +773,33 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_attention_few_kernel(const e
 #pragma unroll
         for (int n = 0; n < NQ; ++n)
 #pragma unroll
-            for (int e = 0; e < NV; ++e) qx[n][e] = p.q[b * p.ldq + (long)(u.h0 + min(n, u.heads - 1)) * DH + i * NV + e] * qs;
+            for (int e = 0; e < NV; ++e) qx[n][e] = p.q[b * p.ldq + (long)(u.h0 + min(n, u.heads - 1)) * DH + feature_of<DH, 4>(i, e)] * qs;
         const int n_tiles = (end - begin + TILE - 1) / TILE;
         const int n_mine = __builtin_amdgcn_readfirstlane(n_tiles > wave ? (n_tiles - wave + NW - 1) / NW : 0);
         const char* kbase = static_cast<const char*>(p.k_cache) + u.hk * p.s_head * 4;
         const char* vbase = static_cast<const char*>(p.v_cache) + u.hk * p.s_head * 4;
         const int row_bytes = (int)(p.s_row * 4);
-        const int lane_at = 4 * g * row_bytes + i * NV * 4;
+        const int lane_at = 4 * g * row_bytes + i * 4 * RUN;
 
         float kr[HALVES][4][NV], vr[HALVES][4][NV];
         [[maybe_unused]] float mk[HALVES][4];
-        auto load = [&](const char* base, float (&r)[HALVES][4][NV]) {
+        auto load = [&](const char* base, float (&r)[HALVES][4][NV], auto hint) {
 #pragma unroll
             for (int s = 0; s < HALVES; ++s)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const char* a = base + walk.at[s] + (unsigned)(lane_at + j * row_bytes);
-                    if constexpr (NV == 2) {
-                        const float2 t = *reinterpret_cast<const float2*>(a);
-                        r[s][j][0] = t.x; r[s][j][1] = t.y;
-                    } else {
+                for (int j = 0; j < 4; ++j)
 #pragma unroll
-                        for (int x = 0; x < NV; x += 4) {
-                            const float4 t = *reinterpret_cast<const float4*>(a + 4 * x);
-                            r[s][j][x] = t.x; r[s][j][x + 1] = t.y; r[s][j][x + 2] = t.z; r[s][j][x + 3] = t.w;
-                        }
+                    for (int x = 0; x < NV; x += RUN) {
+                        const run_t* at = reinterpret_cast<const run_t*>(base + walk.at[s] + (unsigned)(lane_at + 64 * x + j * row_bytes));
+                        run_t t;
+                        if constexpr (decltype(hint)::value) t = __builtin_nontemporal_load(at);
+                        else t = *at;
+#pragma unroll
+                        for (int e = 0; e < RUN; ++e) r[s][j][x + e] = t[e];
                     }
-                }
         };
+        auto load_k = [&]() { load(kbase, kr, std::false_type()); };
+        auto load_v = [&]() { load(vbase, vr, std::bool_constant<STREAM>()); };
         auto load_mask = [&](int it) {
             if constexpr (MASK) {
                 const float* mrow = p.key_mask + b * p.mask_sb;
@@ -806,9 +820,9 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_attention_few_kernel(const e
         }
         if (n_mine > 0) {
             walk.locate(0, false);
-            load(kbase, kr);
+            load_k();
             load_mask(0);
-            load(vbase, vr);
+            load_v();
             for (int it = 0; it < n_mine; ++it) {
                 const int r0 = begin + (it * NW + wave) * TILE;
                 bool ok_now[HALVES], all_in = r0 + TILE <= end;
@@ -841,7 +855,7 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_attention_few_kernel(const e
                 const bool drop = MASK ? (bool)__any(!mine) : !all_in;
                 const int nx = min(it + 1, n_mine - 1);
                 walk.locate(nx, nx != it);
-                load(kbase, kr);
+                load_k();
                 load_mask(nx);
                 if (drop) {
 #pragma unroll
@@ -880,7 +894,7 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_attention_few_kernel(const e
                             for (int e = 0; e < NV; ++e) o[n][e] = fmaf(w, vr[s][j][e], o[n][e]);
                         }
                 }
-                load(vbase, vr);
+                load_v();
             }
         }
 #pragma unroll
@@ -892,7 +906,7 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_attention_few_kernel(const e
             for (int e = 0; e < NV; ++e) {
                 o[n][e] += lane_xor16(o[n][e]);
                 o[n][e] += lane_xor32(o[n][e]);
-                if (g == 0) o_s[wave][n][i * NV + e] = o[n][e];
+                if (g == 0) o_s[wave][n][feature_of<DH, 4>(i, e)] = o[n][e];
             }
         }
         __syncthreads();
@@ -970,12 +984,20 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const estts_paged_atten
 // 131071 rows: 97.8 / 98.4 / 101.8).
 // Requests of up to 1024 rows are not cut: the second launch costs what the shorter sweep gains (4 heads of 64, float32, cut / not cut: one
 // request of 600 rows 7.0 / 6.3 us, of 1000 7.0 / 8.0, of 1500 7.0 / 10.1; and a launch less to issue).  Nor are requests of up to 2048
-// where there is a workgroup for every CU anyway (32 heads on 8 of 128, bfloat16, cut / not cut: 32 requests of 2000 51.8 / 49.0 us, 128 185 /
-// 178, but 128 ragged ones 106 / 112).
+// where there is a workgroup for every CU and no second round of many (32 heads on 8 of 128, bfloat16, cut / not cut: 32 requests of
+// 2000 46.9 / 44.1 us, 32 ragged ones 30.4 / 29.4; but 128 168.9 / 164.3 and 128 ragged ones 98.6 / 106.5, 256 185.8 / 188.6).
 int paged_split_target(int B, int H, int kv_heads, int max_len) {
-    const long per = (long)kv_heads * ((H / kv_heads + 15) / 16);
-    if (max_len <= 1024 || (B * per >= 256 && max_len <= 2048)) return 0;
+    const long per = (long)kv_heads * ((H / kv_heads + 15) / 16), units = B * per;
+    if (max_len <= 1024 || (units >= 256 && units < 1024 && max_len <= 2048)) return 0;
     return per < 256 ? (int)(256 / per) : 1;
+}
+
+// Whether the rows are too many for the 256 MB behind the L2s to hold them until the next call, by the most that the lengths can be.
+// Plain / streaming loads of V: 32 heads on 8 of 128, bfloat16, 32 requests of 1000 rows (131 MB) 26.8 / 23.1 us, of 2000 48.2 / 44.3, 61
+// ragged ones up to 4096 (512 MB) 100.4 / 92.9, one of 131071 (537 MB) 97.4 / 87.7 (6.1 TB/s); 8 heads of 64, float32, 200 of 1021 (836 MB)
+// 146.5 / 138.6 (6.0 TB/s).  But 32 ragged ones up to 1000 (65 MB, called again and again) 16.1 / 17.7 and 8 of 1000 (33 MB) 14.3 / 15.9.
+bool stream_rows(const estts_paged_attention_args& a) {
+    return 2.0 * a.B * a.max_len * a.kv_heads * a.depth * (a.type == ESTTS_KV_F32 ? 4 : 2) > 100e6;
 }
 
 bool bad_cache(const void* k, const void* v, int64_t s_page, int64_t s_head, int64_t s_row, int type, int depth) {
@@ -1050,23 +1072,31 @@ extern "C" int64_t estts_paged_attention_ws_bytes(int32_t B, int32_t H, int32_t 
     return target ? PagedScratch::bytes(target, H, depth, B) : 0;
 }
 
-template <typename T, int DH>
+template <typename T, int DH, bool MASK, bool STREAM>
 static void launch_paged_attention(const estts_paged_attention_args& a, int target, hipStream_t stream) {
     const int group = a.H / a.kv_heads, n_group = (group + 15) / 16;
     const int units = (target ? target : a.B) * a.kv_heads;
     const dim3 grid(n_group > 1 ? (units + 7) / 8 * 8 * n_group : units), block(ATT_WAVES * 64);
     if constexpr (sizeof(T) == 4) {
+        if (group == 1) {
+            ESTTS_LAUNCH((paged_attention_few_kernel<DH, MASK, STREAM, 1, ATT_WAVES>), grid, block, 0, stream, a, target);
+            return;
+        }
         if (group <= FEW_QUERIES) {
-            if (group == 1 && a.key_mask) ESTTS_LAUNCH((paged_attention_few_kernel<DH, true, 1, ATT_WAVES>), grid, block, 0, stream, a, target);
-            else if (group == 1) ESTTS_LAUNCH((paged_attention_few_kernel<DH, false, 1, ATT_WAVES>), grid, block, 0, stream, a, target);
-            else if (a.key_mask) ESTTS_LAUNCH((paged_attention_few_kernel<DH, true, 2, ATT_WAVES>), grid, block, 0, stream, a, target);
-            else ESTTS_LAUNCH((paged_attention_few_kernel<DH, false, 2, ATT_WAVES>), grid, block, 0, stream, a, target);
-            if (target) ESTTS_LAUNCH(paged_join_kernel<DH>, dim3(a.H, a.B), dim3(256), 0, stream, a, target);
+            ESTTS_LAUNCH((paged_attention_few_kernel<DH, MASK, STREAM, FEW_QUERIES, ATT_WAVES>), grid, block, 0, stream, a, target);
             return;
         }
     }
-    if (a.key_mask) ESTTS_LAUNCH((paged_attention_kernel<T, DH, true, ATT_WAVES>), grid, block, 0, stream, a, target);
-    else ESTTS_LAUNCH((paged_attention_kernel<T, DH, false, ATT_WAVES>), grid, block, 0, stream, a, target);
+    ESTTS_LAUNCH((paged_attention_kernel<T, DH, MASK, STREAM, ATT_WAVES>), grid, block, 0, stream, a, target);
+}
+
+template <typename T, int DH>
+static void launch_paged_attention(const estts_paged_attention_args& a, int target, hipStream_t stream) {
+    const bool many = stream_rows(a);
+    if (a.key_mask && many) launch_paged_attention<T, DH, true, true>(a, target, stream);
+    else if (a.key_mask) launch_paged_attention<T, DH, true, false>(a, target, stream);
+    else if (many) launch_paged_attention<T, DH, false, true>(a, target, stream);
+    else launch_paged_attention<T, DH, false, false>(a, target, stream);
     if (target) ESTTS_LAUNCH(paged_join_kernel<DH>, dim3(a.H, a.B), dim3(256), 0, stream, a, target);
 }
 
