@@ -168,11 +168,13 @@ __global__ __launch_bounds__(NT) void page_plan_kernel(const estts_page_plan_arg
 
 template <bool LDS>
 __global__ __launch_bounds__(256) void page_copy_kernel(const estts_page_plan_args p) {
-    __shared__ int plan_s[LDS ? 4 * PLAN_LDS : 1];
+    __shared__ __attribute__((aligned(16))) int plan_s[LDS ? 4 * PLAN_LDS : 4];
     const int* plan = p.ws + PLAN_HEAD;
     const int height0 = p.ws[0], back = p.ws[1], taken = p.ws[2];
     if (LDS) {
-        for (int x = threadIdx.x; x < 4 * p.B; x += 256) plan_s[x] = plan[x];
+        // (four loads in flight: one at a time this was most of the launch)
+#pragma unroll 4
+        for (int x = threadIdx.x; x < p.B; x += 256) reinterpret_cast<int4*>(plan_s)[x] = reinterpret_cast<const int4*>(plan)[x];
         __syncthreads();
         plan = plan_s;
     }
@@ -1045,7 +1047,8 @@ extern "C" int estts_page_plan(const estts_page_plan_args* args, void* stream) {
     ESTTS_CHECK_ARG((int64_t)a.P * a.page < (1LL << 31) && (int64_t)a.n_pages * a.page < (1LL << 31) && (int64_t)a.B * a.P < (1LL << 31),
                     "estts_page_plan: P * page, n_pages * page and B * P must stay below 2^31");
     const int64_t need = estts_page_plan_ws_bytes(a.B, a.T);
-    ESTTS_CHECK_ARG(need == 0 || (a.ws && a.ws_bytes >= need), "estts_page_plan: this call needs %ld bytes of scratch (given: %ld)", (long)need, (long)a.ws_bytes);
+    ESTTS_CHECK_ARG(need == 0 || (a.ws && a.ws_bytes >= need && !(reinterpret_cast<uintptr_t>(a.ws) & 15)),
+                    "estts_page_plan: this call needs %ld bytes of scratch, 16-byte aligned (given: %ld)", (long)need, (long)a.ws_bytes);
     const hipStream_t st = (hipStream_t)stream;
     const int split = a.T > PLAN_ROWS;
     if (a.B > PLAN_LDS) ESTTS_LAUNCH((page_plan_kernel<1024, false>), dim3(1), dim3(1024), 0, st, a, split);

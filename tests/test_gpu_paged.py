@@ -216,6 +216,26 @@ def test_page_write_is_exact(kind, order, T, Hk, D, page):
         assert torch.equal(torch.isnan(a), torch.isnan(b)) and torch.equal(torch.nan_to_num(a, nan=3.0), torch.nan_to_num(b, nan=3.0))
 
 
+@pytest.mark.parametrize('kind', sorted(TYPES))
+@pytest.mark.parametrize('T,Hk,D,order', [(9000, 8, 64, 'head'), (4001, 12, 128, 'token'), (70000, 1, 72, 'gaps')])
+def test_page_write_of_many_rows(kind, T, Hk, D, order):
+    """Writes large enough for streaming stores, against one assignment."""
+    page = 32
+    n_pages = T // page + 9
+    kc, vc = cache_pair(n_pages, page, Hk, D, TYPES[kind], order)
+    g = torch.Generator(device=DEV).manual_seed(T)
+    rows = torch.randn(T, 2 * Hk * D, generator=g, device=DEV)
+    slots = torch.randperm(n_pages * page, generator=g, device=DEV)[:T]
+    slots[5::17] = -1
+    want = []
+    for x, c in ((rows[:, :Hk * D], kc), (rows[:, Hk * D:], vc)):
+        w = c.clone(memory_format=torch.contiguous_format).transpose(1, 2).reshape(-1, Hk, D)
+        w[slots[slots >= 0]] = x[slots >= 0].reshape(-1, Hk, D).to(TYPES[kind])
+        want.append(w.view(n_pages, page, Hk, D).transpose(1, 2))
+    ops.page_write(rows[:, :Hk * D], rows[:, Hk * D:], kc, vc, slots.int())
+    assert torch.equal(kc, want[0]) and torch.equal(vc, want[1])
+
+
 def test_page_write_leaves_gaps_alone():
     base = [torch.full((6, 3, 19, 80), 5.0, device=DEV) for _ in range(2)]
     kc, vc = (c[:, :2, :16, :64] for c in base)
@@ -277,11 +297,15 @@ def pages_for(lengths, page, g, P=None, spare=3):
     return table, n_pages
 
 
-def check_attention(lengths, heads, Hk, D, page, kind, mask=None, order='head', scale=None, max_len=None, spoil=None, seed=0, spread=1.0):
+def check_attention(lengths, heads, Hk, D, page, kind, mask=None, order='head', scale=None, max_len=None, spoil=None, seed=0, spread=1.0, P=None,
+                    cache_scale=1.0):
     g = torch.Generator().manual_seed(seed)
     B = len(lengths)
-    table, n_pages = pages_for(lengths, page, g)
+    table, n_pages = pages_for(lengths, page, g, P)
     kc, vc = cache_pair(n_pages, page, Hk, D, TYPES[kind], order, seed)
+    if cache_scale != 1.0:
+        most = torch.finfo(kc.dtype).max                  # (a normal value 3.3 times 2e4 would be an infinity in float16)
+        kc, vc = ((c.float() * cache_scale).clamp(-most, most).to(c.dtype) for c in (kc, vc))
     q = (torch.randn(B, heads * D + 8, generator=g) * spread).to(DEV)[:, :heads * D]
     P = table.shape[1]
     if spoil is not None:
@@ -320,6 +344,39 @@ def test_attention_over_long_requests(kind, heads, Hk, D, page, lengths):
 def test_attention_of_many_requests(kind, B):
     g = torch.Generator().manual_seed(B)
     check_attention(torch.randint(0, 400, (B,), generator=g).tolist(), 4, 2, 32, 16, kind, seed=B)
+
+
+@pytest.mark.parametrize('kind', sorted(TYPES))
+@pytest.mark.parametrize('B', [3, 257, 1000])
+def test_attention_of_many_requests_beside_long_ones(kind, B):
+    """The line of all rows cut into parts: many requests to a part, several parts to a request, requests without rows."""
+    g = torch.Generator().manual_seed(B)
+    lengths = torch.randint(0, 90, (B,), generator=g).tolist()
+    lengths[B // 2], lengths[0], lengths[-1] = 2600, 1100, 0
+    check_attention(lengths, 4, 2, 64, 16, kind, seed=B)
+
+
+@pytest.mark.parametrize('kind', sorted(TYPES))
+@pytest.mark.parametrize('D', [32, 64, 128])
+@pytest.mark.parametrize('heads,Hk', [(4, 4), (8, 4), (24, 4), (80, 4)])
+@pytest.mark.parametrize('masked', [False, True])
+def test_attention_when_the_rows_could_be_many(kind, D, heads, Hk, masked):
+    """A bound on the lengths of more than 100 MB of rows: the kernels whose loads of V stream past the caches."""
+    lengths = [0, 1, 16, 33, 100, 1300, 517, 64]
+    P = 32768 // 16 if D * (4 if kind == 'f32' else 2) < 256 else 16384 // 16
+    assert 2 * len(lengths) * P * 16 * Hk * D * (4 if kind == 'f32' else 2) > 100e6
+    mask = None
+    if masked:
+        mask = (torch.rand(len(lengths), P * 16, generator=torch.Generator().manual_seed(D)) < 0.3).float()
+        mask[3] = 1.0
+    check_attention(lengths, heads, Hk, D, 16, kind, mask=mask, seed=D, P=P)
+
+
+@pytest.mark.parametrize('kind,cache_scale', [('f16', 1e-6), ('f16', 2e4), ('bf16', 1e-30), ('bf16', 1e30), ('f32', 1e-30), ('f32', 1e30)])
+@pytest.mark.parametrize('heads', [2, 6])
+def test_attention_over_the_range_of_the_cache_types(kind, cache_scale, heads):
+    """float16 subnormals and values near its end; scores kept moderate by the scale."""
+    check_attention([90, 1400], heads, 2, 64, 16, kind, scale=0.1 / cache_scale if cache_scale < 1e20 else 1e-31, cache_scale=cache_scale, seed=12)
 
 
 @pytest.mark.parametrize('kind', sorted(TYPES))

@@ -147,3 +147,120 @@ def test_pages_must_be_a_multiple_of_sixteen_rows():
     lib = _lib.load()
     for page in (1, 8, 15, 17, 40):
         assert lib.estts_page_plan(plan_block(page=page), None) != 0 and b'multiple of 16' in lib.estts_last_error()
+
+
+# ------------------------------------------------------------------------------------------- models of the kernels' index arithmetic
+# The formulas restate csrc/paged.hip; a kernel change that moves an index has to move it here too.
+def request_rows(length, P, page, max_len):
+    return min(max(length, 0), P * page, max_len)
+
+
+def parts_of(lengths, target, unit):
+    """PagedPart: for every part the segments (request, first unit, units, units of the request, place or None) it works through, and
+    where the join finds each request (first part, number of parts)."""
+    units = [max(-(-n // unit), 1) for n in lengths]
+    total = sum(units)
+    n_parts = min(target, total)
+    line, parts, items = 0, [], {}
+    starts = []
+    for n in units:
+        starts.append(line)
+        line += n
+    for k in range(n_parts):
+        lo, hi = k * total // n_parts, (k + 1) * total // n_parts
+        b = max(i for i, s in enumerate(starts) if s <= lo)
+        off, left, at, segments = lo - starts[b], hi - lo, lo, []
+        while left > 0:
+            take = min(units[b] - off, left)
+            whole = take == units[b]
+            segments.append((b, off, take, units[b], None if whole else 2 * k + (off == 0)))
+            if off == 0:
+                items[b] = (k, 1 if whole else ((at + units[b]) * n_parts - 1) // total - k + 1)
+            left, at, off, b = left - take, at + take, 0, b + 1
+        parts.append(segments)
+    return parts, items
+
+
+@pytest.mark.parametrize('lengths', [[0], [1], [131071], [5000, 0, 0, 1, 300, 128, 129], [100] * 300, [0] * 7, [3000] + [1] * 700 + [2500], list(range(0, 4000, 37))])
+@pytest.mark.parametrize('target', [1, 2, 32, 64, 256])
+@pytest.mark.parametrize('unit', [64, 128])
+def test_parts_cover_every_row_once_and_the_join_finds_them(lengths, target, unit):
+    parts, items = parts_of(lengths, target, unit)
+    seen, places = {}, {}
+    for k, segments in enumerate(parts):
+        assert segments
+        for b, off, take, n, place in segments:
+            for u in range(off, off + take):
+                assert (b, u) not in seen
+                seen[b, u] = k
+            if place is not None:
+                assert 0 <= place < 2 * target and place not in places          # (two places a part, each used once)
+                places[place] = b
+    for b, rows in enumerate(lengths):
+        n = max(-(-rows // unit), 1)
+        assert all((b, u) in seen for u in range(n)) and (b, n) not in seen
+        first, count = items[b]
+        assert (first, count) == (seen[b, 0], seen[b, n - 1] - seen[b, 0] + 1)
+        if count > 1:                               # what paged_join_kernel reads
+            read = [2 * first + 1] + [2 * (first + s) for s in range(1, count)]
+            assert [places[x] for x in read] == [b] * count
+    # equal parts: no two differ by more than a unit
+    sizes = [sum(t for _, _, t, _, _ in s) for s in parts]
+    assert max(sizes) - min(sizes) <= 1
+
+
+@pytest.mark.parametrize('halves,waves', [(1, 4), (2, 4)])
+@pytest.mark.parametrize('page', [16, 48, 64])
+@pytest.mark.parametrize('P,max_len,begin,end', [(1, 16, 0, 1), (3, 40, 0, 40), (70, 1000, 0, 1000), (70, 1111, 512, 1111), (700, 9000, 4096, 9000)])
+def test_page_walk_stays_inside_table_and_pages(halves, waves, page, P, max_len, begin, end):
+    """Every table entry that PageWalk reads lies in the request's row of the table, every half of a tile in one page, and the lanes hold
+    the half that locate() asks for."""
+    max_len = min(max_len, P * page)
+    end = min(end, max_len)
+    tile, per_block = 16 * halves, 64 // halves
+    n_tiles = max(-(-(end - begin) // tile), 0)
+    half_row = lambda block, lane, wave: begin + ((block * per_block + lane // halves) * waves + wave) * tile + 16 * (lane % halves)
+    for wave in range(waves):
+        mine = (n_tiles - wave + waves - 1) // waves if n_tiles > wave else 0
+        for block in range(max(mine - 1, 0) // per_block + 3):
+            for lane in (0, 1, 2, 31, 62, 63):
+                assert 0 <= min(half_row(block, lane, wave), max_len - 1) // page < P
+        for it in range(mine):
+            for s in range(halves):
+                lane = (it % per_block) * halves + s
+                r = half_row(it // per_block, lane, wave)
+                assert r == begin + (it * waves + wave) * tile + 16 * s
+                assert r % page + 15 < page or r % page + 16 == page           # (sixteen rows of one page)
+
+
+@pytest.mark.parametrize('entry', [-2 ** 31, -1, 7, 8, 2 ** 31 - 1])
+def test_pages_and_slots_that_do_not_exist_reach_no_memory(entry):
+    """place() and page_write_kernel: an id or slot outside the cache is never turned into an address."""
+    n_pages, page = 7, 16
+    there = 0 <= entry < n_pages
+    assert not there                                                            # (place: offset -1, locate: row 0 of page 0, rows left out)
+    for slot in (entry, entry & 0xFFFFFFFF):
+        assert (slot & 0xFFFFFFFF) >= n_pages * page or 0 <= slot < n_pages * page
+    assert ((-1) & 0xFFFFFFFF) >= n_pages * page
+
+
+@pytest.mark.parametrize('depth,esize', [(32, 2), (64, 2), (128, 2), (32, 4), (64, 4), (128, 4)])
+def test_lane_loads_cover_each_row_once(depth, esize):
+    """feature_of and the byte offsets of the loads: the 16 lanes of a row read every byte of it once, and element e of lane r is feature
+    feature_of(r, e); of K, lane (i, g) of load x reads bytes 16 g + 64 x .. + 15."""
+    nv = depth // 16
+    run = nv if nv * esize < 16 else 16 // esize
+    feature = lambda r, e: (e // run) * (16 * run) + r * run + e % run
+    assert sorted(feature(r, e) for r in range(16) for e in range(nv)) == list(range(depth))
+    for r in range(16):
+        for e in range(nv):
+            load = e // run
+            assert feature(r, e) * esize == r * run * esize + 256 * load + (e % run) * esize
+    k_bytes = sorted(b for g in range(4) for x in range(depth * esize // 64) for b in range(16 * g + 64 * x, 16 * g + 64 * x + 16))
+    assert k_bytes == list(range(depth * esize))
+    # buffer range of a half: the last byte read is the last of its sixteenth row
+    row_bytes = depth * esize + 32
+    half_bytes = 15 * row_bytes + depth * esize
+    last_v = 4 * 3 * row_bytes + 15 * run * esize + 256 * ((nv - 1) // run) + 3 * row_bytes + run * esize
+    last_k = 15 * row_bytes + 16 * 3 + 64 * (depth * esize // 64 - 1) + 16
+    assert last_v == last_k == half_bytes
