@@ -9,7 +9,9 @@ namespace {
 // ------------------------------------------------------------------------------------------------ page plan
 // Whole-number work on a few kilobytes, bound by latency: a launch, the lengths, the scans, the stack or the table, the maps.  One
 // workgroup scans the requests; the copies and the rows' places are then made by the same workgroup, or by a second launch
-// of as many as it takes where there are more of them than PLAN_ROWS.
+// of as many as it takes where there are more than PLAN_ROWS rows (one workgroup for all: 64 prompts of 2047 rows at most 95 us, now 8.6;
+// 1000 requests that end, grow and arrive, 26000 rows, 84 us, now 14).  A step of 32 requests is one launch of 4.3 us, some 2 of which are
+// the launch itself.
 constexpr int PLAN_LDS = 4096;         // requests whose plan fits the LDS (four ints each); beyond that it lives in the caller's scratch
 
 __device__ __forceinline__ int pages_of(int rows, int page) { return (int)(((unsigned)rows + page - 1) / (unsigned)page); }
@@ -237,10 +239,13 @@ __global__ __launch_bounds__(256) void page_write_kernel(const estts_page_write_
 // the queries and the weights are split into bfloat16 pieces (three, 24 bits) or float16 pieces (two, 22 bits, behind a power of two that
 // puts the largest element of the query at 2^13 and the largest weight at 2^14), whose products with the pages' values are exact.
 // Scores, maxima, sums and outputs are float32.
+// What bounds it: memory where there are rows enough (5.9 to 6.2 TB/s from 130 MB on; a kernel that only reads gets 6.2), else the chain
+// launch, lengths and table, keys, scores, weights, values, exchange (4.5 us for one request of 100 rows) and some 0.6 to 1.1 us more for
+// each further tile of a wave.
 
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
 
-constexpr int ATT_WAVES = 4;           // waves of a workgroup (8 and 16 gain nothing: a wave's arithmetic fills its SIMD's share)
+constexpr int ATT_WAVES = 4;           // waves of a workgroup (8: 61 ragged requests 92.8 -> 98.4 us, 8 of 1000 rows 14.4 -> 15.8)
 constexpr int FEW_QUERIES = 2;         // query heads per key head up to which float32 pages take the vector ALU
 
 // 16-row halves of a wave's tile
@@ -495,7 +500,7 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_attention_kernel(const estts
         const float qs = p.scale * 1.4426950408889634f;
         const bool live = i < heads;
         const float* qp = p.q + b * p.ldq + (long)(h0 + (live ? i : 0)) * DH;
-        constexpr int QV = F32 ? DH / 4 : DH / 4;           // elements of the query per lane
+        constexpr int QV = DH / 4;                          // elements of the query per lane
         float qx[QV];
 #pragma unroll
         for (int s = 0; s < QV / 4; ++s) {
@@ -519,17 +524,14 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_attention_kernel(const estts
 #pragma unroll
             for (int e = 0; e < QV; ++e) qx[e] *= up;
         }
-        [[maybe_unused]] typename Kv16<typename std::conditional<F32, __bf16, T>::type>::Frag qf[F32 ? 1 : DH / 32][3];
+        [[maybe_unused]] typename Kv16<typename std::conditional<F32, __bf16, T>::type>::Frag qf[F32 ? 1 : DH / 32][Kv16<T>::PIECES];
         if constexpr (!F32) {
 #pragma unroll
             for (int s = 0; s < DH / 32; ++s) {
                 float t[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) t[e] = qx[8 * s + e];
-                typename Kv16<T>::Frag f[Kv16<T>::PIECES];
-                split_pieces<T>(t, f);
-#pragma unroll
-                for (int n = 0; n < Kv16<T>::PIECES; ++n) qf[s][n] = f[n];
+                split_pieces<T>(t, qf[s]);
             }
         }
 
@@ -592,7 +594,7 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_attention_kernel(const estts
 #pragma unroll
         for (int e = 0; e < NV; ++e) o[e] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
         float m = -INFINITY, l = 0.0f;                      // of query i; l: this lane's rows only
-        constexpr float LIFT = !F32 && sizeof(T) == 2 && std::is_same<T, _Float16>::value ? 14.0f : 0.0f;
+        constexpr float LIFT = std::is_same<T, _Float16>::value ? 14.0f : 0.0f;      // (the power of two on the weights)
 
         if (n_mine > 0) {
             walk.locate(0, false);
@@ -1000,9 +1002,9 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const estts_paged_atten
 }
 
 // How many parts a call is cut into (0: one workgroup per request and key head, one launch).
-// Parts: one workgroup per CU.  Its four waves keep 64 KB of keys and values in flight; twice and four times as many workgroups
-// measured the same or less (61 ragged requests up to 4096 rows of bfloat16: 102.2 / 103.0 / 104.5 us with 256 / 512 / 1024; one request of
-// 131071 rows: 97.8 / 98.4 / 101.8).
+// Parts: one workgroup per CU.  Its four waves keep 64 KB of keys and values in flight, and more parts are more ends to join (256 / 512 / 1024
+// parts over all key heads: 61 ragged requests up to 4096 rows of bfloat16 92.8 / 94.7 / 99.7 us, one of 131071 rows 87.0 / 89.4 / 94.4; 128
+// leave half of the CUs idle: 123.8 and 107.0).
 // Requests of up to 1024 rows are not cut: the second launch costs what the shorter sweep gains (4 heads of 64, float32, cut / not cut: one
 // request of 600 rows 7.0 / 6.3 us, of 1000 7.0 / 8.0, of 1500 7.0 / 10.1; and a launch less to issue).  Nor are requests of up to 2048
 // where there is a workgroup for every CU and no second round of many (32 heads on 8 of 128, bfloat16, cut / not cut: 32 requests of

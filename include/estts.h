@@ -944,9 +944,10 @@ int estts_page_write(const estts_page_write_args* args, void* stream);
  *   s_j = scale q[b, h] . k_j   for the rows j < min(lengths[b], max_len) with key_mask[b, j] == 0
  *   ctx[b, h] = sum_j softmax(s)_j v_j;   a request without such rows gets zeros
  * q [B, H depth] and ctx [B, H depth] float32 (row strides ldq, ldo), H a multiple of kv_heads: query head h reads key head
- * h / (H / kv_heads).  depth 32, 64 or 128.  key_mask (may be NULL) float32 with strides mask_sb (request) and mask_ss (position): any value
- * but 0 leaves the row out, whatever the row holds (estts_attention adds -1e9 instead, so that a fully masked row there is a
- * mean of the values).  max_len bounds the lengths (0: P page); it decides how the work is split, and a low bound lets short
+ * h / (H / kv_heads).  depth 32, 64 or 128.  key_mask (may be NULL) float32 with strides mask_sb (request) and mask_ss (position), max_len
+ * positions a request: any value but 0 leaves the row out, whatever the row holds, as rows behind the length are left out
+ * (estts_attention adds -1e9 instead, so that a fully masked row there is a mean of the values).  The rows that count and the
+ * queries are finite (an infinity among them may come out as NaN).  max_len bounds the lengths (0: P page); it decides how the work is split, and a low bound lets short
  * requests run in one launch.  Products and sums have float32 accuracy for every cache type.
  * ws: estts_paged_attention_ws_bytes() bytes (may be NULL where that is 0) that belong to this call until it has run. */
 typedef struct estts_paged_attention_args {
