@@ -304,6 +304,30 @@ def load():
     return lib
 
 
+_host = None
+
+
+def load_host(scratch):
+    """The C module that issues the paged-decoding operators (csrc/hostops.c), set up with this library's entry points and torch's
+    device and stream queries; raise if it is not built.  scratch(nbytes, device): a tensor for one launch."""
+    global _host
+    if _host is None:
+        lib = load()
+        import torch
+        from importlib import machinery, util
+        path = os.path.join(_PKG, '_hostops.so')
+        if not os.path.exists(path):
+            raise EsttsError(f'{path} not found: the extension is not built (make -C {_PKG}/csrc)')
+        spec = util.spec_from_file_location('_hostops', path, loader=machinery.ExtensionFileLoader('_hostops', path))
+        mod = util.module_from_spec(spec)
+        spec.loader.exec_module(mod)
+        at = [C.cast(getattr(lib, n), _vp).value for n in ('estts_page_plan', 'estts_page_write', 'estts_paged_attention', 'estts_page_plan_ws_bytes',
+                                                           'estts_paged_attention_ws_bytes')]
+        mod.setup(*at, scratch, torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream, torch.int32, torch.float32, torch.bfloat16, torch.float16)
+        _host = mod
+    return _host
+
+
 def check(rc, what):
     if rc != 0:
         msg = load().estts_last_error()

@@ -690,6 +690,14 @@ def _check_pages(what, k_cache, v_cache):
     raise ValueError(f'{what}: k_cache and v_cache must be [n_pages, kv_heads, page, depth] tensors of the same strides and type')
 
 
+def _issue():
+    """The C module that issues plain calls of the operators below, None while launches are recorded, traced or named: those, and whatever
+    the module turns down, take the Python path behind it, which says what is wrong."""
+    if _program is not None or _trace is not None or _debug_sync:
+        return None
+    return _lib._host or _lib.load_host(_scratch)
+
+
 def new_paged_cache(n_pages, page, kv_heads, depth, dtype=torch.float32, device='cuda'):
     """(k_cache, v_cache) of n_pages pages of `page` rows (a multiple of 16) each, for page_write / paged_attention."""
     return tuple(torch.zeros(n_pages, kv_heads, page, depth, dtype=dtype, device=device) for _ in range(2))
@@ -705,6 +713,9 @@ def page_plan(lengths, new, block_table, free_pages, n_free, page, slots, positi
     is read back by the host, so a captured step plans itself anew on every replay."""
     lengths_out = lengths if lengths_out is None else lengths_out
     n_free_out = n_free if n_free_out is None else n_free_out
+    host = _issue()
+    if host is not None and host.page_plan(lengths, new, block_table, free_pages, n_free, page, slots, positions, lengths_out, n_free_out, refused):
+        return slots
     B, T, padded = lengths.numel(), slots.numel(), slots.dim() == 2
     _check_i32('page_plan', lengths, 'lengths', (B,))
     _check_i32('page_plan', new, 'new', (B,))
@@ -744,6 +755,9 @@ def page_write(k, v, k_cache, v_cache, slots):
     """Rows k, v ([T, >= kv_heads * depth] float32 views, head after head) into the pages (estts_page_write): row t goes to slots[t]
     (int32, any shape with T elements; page * page size + row, what page_plan writes), rounded to the caches' type; rows with a
     slot outside the cache go nowhere.  The slots of a call must be distinct."""
+    host = _issue()
+    if host is not None and host.page_write(k, v, k_cache, v_cache, slots):
+        return
     (n_pages, Hk, page, D), (s_page, s_head, s_row, _) = _check_pages('page_write', k_cache, v_cache)
     if (n_pages > 1 and not s_page) or (Hk > 1 and not s_head) or not s_row:
         raise ValueError('page_write: the caches must not be broadcast views')
@@ -770,6 +784,9 @@ def paged_attention(q, k_cache, v_cache, block_table, lengths, ctx, heads, key_m
     page_plan leaves them (the new row is in its page already).  key_mask: [B, >= max_len] float32 view, rows with any value but 0 are
     left out; a request with nothing left gets zeros.  scale: 1 / sqrt(depth) if None.  max_len: bound on the lengths that the host
     knows of (P * page if None; rows past it are not read)."""
+    host = _issue()
+    if host is not None and host.paged_attention(q, k_cache, v_cache, block_table, lengths, ctx, heads, key_mask, scale, max_len):
+        return ctx
     B = lengths.numel()
     (n_pages, Hk, page, D), (s_page, s_head, s_row, _) = _check_pages('paged_attention', k_cache, v_cache)
     _check_i32('paged_attention', lengths, 'lengths', (B,))

@@ -646,3 +646,89 @@ def test_a_step_program_issues_the_three_operators():
         direct(i)
     assert torch.equal(outs[0], outs[1]) and bool((outs[0].abs().sum(-1) > 0).all())
     assert one.lengths.tolist() == [steps] * one.B
+
+
+# -------------------------------------------------------------------------------------------------- the two ways to issue a call
+def python_path(monkeypatch):
+    monkeypatch.setattr(ops, '_issue', lambda: None)
+
+
+@pytest.mark.parametrize('kind', sorted(TYPES))
+def test_the_c_module_and_the_python_path_issue_the_same_launches(monkeypatch, kind):
+    """A loop through csrc/hostops.c and one through the Python path: the same bits everywhere.  While the first runs the argument blocks of
+    the second are out of reach, so that it cannot have taken that path."""
+    width, steps = Loop(kind).qkv.shape[1], 24
+    plan = feeds(5, width, steps, 21)
+    blocks = {n: getattr(ops._lib, n) for n in ('PagePlanArgs', 'PageWriteArgs', 'PagedAttentionArgs')}
+    loops = []
+    for fast in (True, False):
+        with monkeypatch.context() as mp:
+            if fast:
+                for n in blocks:
+                    mp.setattr(ops._lib, n, None)
+            else:
+                python_path(mp)
+            loop = Loop(kind, P=130, n_pages=700)
+            big = torch.randn(5 * 1300, 2 * loop.Hk * loop.D, generator=torch.Generator().manual_seed(1)).to(DEV)
+            slots, positions, refused = (torch.empty(s, dtype=torch.int32, device=DEV) for s in ((6513,), (6513,), (1,)))
+            ops.page_plan(loop.lengths, dev([1300, 700, 0, 1300, 1200]), loop.table, loop.free, loop.n_free, loop.page, slots, positions=positions,
+                          refused=refused)
+            ops.page_write(big[:, :loop.Hk * loop.D], big[:, loop.Hk * loop.D:], loop.kc, loop.vc, slots[:6500])
+            seen = []
+            for rows, new in plan:
+                loop.qkv.copy_(rows)
+                loop.new.copy_(new)
+                loop.step()
+                masked = ops.paged_attention(loop.qkv[:, :loop.H * loop.D], loop.kc, loop.vc, loop.table, loop.lengths, torch.zeros_like(loop.ctx), loop.H,
+                                             key_mask=(torch.arange(2080, device=DEV) % 3 == 1).float().expand(5, 2080), scale=0.2, max_len=1900)
+                seen += [loop.ctx.clone(), masked, loop.lengths.clone(), loop.slots.clone()]
+            loops.append(seen + [slots, positions, refused, loop.table, loop.free, loop.n_free, loop.kc, loop.vc])
+    assert all(torch.equal(a, b) for a, b in zip(*loops)) and len(loops[0]) == len(loops[1])
+
+
+def good_calls():
+    g = torch.Generator().manual_seed(3)
+    kc, vc = cache_pair(12, 16, 2, 64, torch.float32)
+    kc16, _ = cache_pair(12, 16, 2, 64, torch.float16)
+    q, rows = torch.randn(3, 256, generator=g).to(DEV), torch.randn(3, 128, generator=g).to(DEV)
+    i32 = lambda *s: torch.zeros(*s, dtype=torch.int32, device=DEV)
+    attend = dict(q=q, k_cache=kc, v_cache=vc, block_table=i32(3, 4), lengths=i32(3), ctx=torch.zeros(3, 256, device=DEV), heads=4)
+    write = dict(k=rows, v=rows, k_cache=kc, v_cache=vc, slots=i32(3))
+    plan = dict(lengths=i32(3), new=i32(3), block_table=i32(3, 4), free_pages=i32(12), n_free=i32(1), page=16, slots=i32(3, 1))
+    f = lambda *s: torch.zeros(*s, device=DEV)
+    bad = [(ops.paged_attention, attend, b) for b in (
+        dict(q=q.half()), dict(q=q[:, :255]), dict(q=q.t()), dict(q=q.cpu()), dict(ctx=f(2, 256)), dict(ctx=f(3, 256).cpu()), dict(heads=3), dict(heads=0),
+        dict(k_cache=kc16), dict(k_cache=kc16.double(), v_cache=kc16.double()), dict(k_cache=kc[:, :, :, ::2], v_cache=vc[:, :, :, ::2]),
+        dict(v_cache=vc[:5]), dict(block_table=i32(4, 4)), dict(block_table=i32(4, 3).t()), dict(block_table=i32(3, 4).long()), dict(lengths=i32(3).long()),
+        dict(lengths=i32(6)[::2]), dict(key_mask=f(3, 63)), dict(key_mask=f(3, 64).bool()), dict(key_mask=f(3, 64).cpu()), dict(max_len=0), dict(max_len=-5),
+        dict(k_cache=kc[:, :, :8], v_cache=vc[:, :, :8]), dict(q=f(3, 257)[:, 1:]))]
+    bad += [(ops.page_write, write, b) for b in (
+        dict(k=rows[:2]), dict(v=rows[:, :100]), dict(k=rows.half()), dict(slots=i32(4)), dict(slots=i32(3).long()), dict(slots=i32(6)[::2]), dict(slots=i32(3).cpu()),
+        dict(k_cache=kc[:1].expand(12, 2, 16, 64), v_cache=vc[:1].expand(12, 2, 16, 64)), dict(k_cache=kc16), dict(k=f(3, 129)[:, 1:]), dict(k_cache=kc[:, :, :5], v_cache=vc[:, :, :5]))]
+    bad += [(ops.page_plan, plan, b) for b in (
+        dict(new=i32(4)), dict(new=i32(3).long()), dict(block_table=i32(2, 4)), dict(free_pages=i32(12).cpu()), dict(n_free=i32(2)), dict(page=8), dict(page=-16),
+        dict(slots=i32(2, 1)), dict(slots=i32(3, 2)[:, :1]), dict(slots=i32(1, 3, 1)), dict(positions=i32(3)), dict(lengths_out=i32(4)), dict(n_free_out=i32(3)),
+        dict(refused=f(1)), dict(lengths=i32(3).cpu()))]
+    return bad
+
+
+@pytest.mark.parametrize('python', [False, True])
+def test_both_ways_refuse_the_same_calls(monkeypatch, python):
+    if python:
+        python_path(monkeypatch)
+    for fn, good, bad in good_calls():
+        fn(**good)
+        with pytest.raises((ValueError, TypeError, ops._lib.EsttsError)):
+            fn(**dict(good, **bad))
+            raise AssertionError(f'{fn.__name__} took {[(k, getattr(v, "shape", v)) for k, v in bad.items()]}')
+
+
+def test_calls_the_c_module_leaves_to_python_work(monkeypatch):
+    """Sizes and scales that are not plain Python numbers, one-row views with any stride, caches with dimensions of one."""
+    kc, vc = cache_pair(1, 16, 1, 64, torch.float32)
+    q = torch.randn(1, 300, device=DEV)[:, :64]
+    args = (kc, vc, torch.zeros(1, 1, dtype=torch.int32, device=DEV), dev([9]))
+    a = ops.paged_attention(q, *args, torch.empty(1, 64, device=DEV), 1, scale=1, max_len=16)
+    b = ops.paged_attention(q, *args, torch.empty(1, 64, device=DEV), 1, scale=1.0, max_len=16.0)
+    python_path(monkeypatch)
+    assert torch.equal(a, b) and torch.equal(a, ops.paged_attention(q, *args, torch.empty(1, 64, device=DEV), 1, scale=1.0))
