@@ -447,6 +447,16 @@ struct PagedUnit {
     }
 };
 
+// The rows of a tile that count, a bit for each: in range, in a page that exists, not masked.  A lane looks at one row (mask: of row
+// lane % TILE), the wave holds the answer.
+template <int HALVES>
+__device__ __forceinline__ uint32_t rows_that_count(int r0, int end, const bool (&ok)[HALVES], float mask) {
+    const int row = threadIdx.x % (16 * HALVES);
+    const bool there = HALVES == 2 && row >= 16 ? ok[HALVES - 1] : ok[0];
+    const uint64_t bits = __ballot(there && r0 + row < end && mask == 0.0f);
+    return HALVES == 2 ? (uint32_t)bits : (uint32_t)bits & 0xFFFFu;
+}
+
 // The waves' shares (o_s, m_s, l_s in the LDS) meet; to ctx, or to the scratch where the segment is not a whole request.
 template <int NW, int MAXQ, int DH>
 __device__ __forceinline__ void join_waves(const estts_paged_attention_args& p, const PagedUnit<MAXQ>& u, const PagedSegment& seg, const PagedScratch& ws,
@@ -479,6 +489,7 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_attention_kernel(const estts
     constexpr bool F32 = sizeof(T) == 4;
     constexpr int HALVES = tile_halves(DH, sizeof(T));
     constexpr int TILE = 16 * HALVES;
+    constexpr uint32_t ALL_ROWS = HALVES == 2 ? 0xFFFFFFFFu : 0xFFFFu;
     constexpr int NV = DH / 16;                         // features of a row of V per lane = tiles of 16 features
     constexpr int VB = NV * (int)sizeof(T) < 16 ? NV * (int)sizeof(T) : 16;     // bytes of one load of them
     __shared__ __attribute__((aligned(16))) float o_s[NW][16][DH];
@@ -547,7 +558,7 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_attention_kernel(const estts
         constexpr int VW = NV * (int)sizeof(T) / 4;         // dwords of V per row and lane
         i32x4 kr[HALVES][KL];
         int vr[HALVES][4][VW];
-        [[maybe_unused]] float mk[HALVES][4];
+        [[maybe_unused]] float mk;                          // mask of row lane % TILE of the tile
         const int k_lane = i * row_bytes + 16 * g;
         const int v_lane = 4 * g * row_bytes + i * VB;
         const int half_bytes = 15 * row_bytes + DH * (int)sizeof(T);
@@ -558,14 +569,7 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_attention_kernel(const estts
 #pragma unroll
                 for (int x = 0; x < KL; ++x) kr[s][x] = __builtin_amdgcn_raw_buffer_load_b128(rows, k_lane + 64 * x, 0, 0);
             }
-            if constexpr (MASK) {
-                const float* mrow = p.key_mask + b * p.mask_sb;
-                const int r0 = begin + (it * NW + wave) * TILE + 4 * g;
-#pragma unroll
-                for (int s = 0; s < HALVES; ++s)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) mk[s][j] = mrow[min(r0 + 16 * s + j, end - 1) * p.mask_ss];
-            }
+            if constexpr (MASK) mk = p.key_mask[b * p.mask_sb + min(begin + (it * NW + wave) * TILE + lane % TILE, end - 1) * p.mask_ss];
         };
         constexpr int POLICY = STREAM ? LOAD_STREAM : 0;
         auto load_v = [&]() {
@@ -649,24 +653,11 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_attention_kernel(const estts
                 bool all_in = r0 + TILE <= end;
 #pragma unroll
                 for (int s = 0; s < HALVES; ++s) all_in = all_in && ok_now[s];
-                bool in[HALVES][4], drop = !all_in;
-                auto find_in = [&]() {
-#pragma unroll
-                    for (int s = 0; s < HALVES; ++s)
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            in[s][j] = ok_now[s] && r0 + 16 * s + 4 * g + j < end;
-                            if constexpr (MASK) in[s][j] = in[s][j] && mk[s][j] == 0.0f;
-                        }
-                };
-                if constexpr (MASK) {
-                    find_in();
-                    bool mine = true;
-#pragma unroll
-                    for (int s = 0; s < HALVES; ++s)
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) mine = mine && in[s][j];
-                    drop = __any(!mine);
+                uint32_t rows_in = 0;                       // a bit for each
+                bool drop = !all_in;
+                if (MASK || drop) {
+                    rows_in = rows_that_count<HALVES>(r0, end, ok_now, MASK ? mk : 0.0f);
+                    drop = rows_in != ALL_ROWS;
                 }
                 // the next tile's keys, into the registers just read (the last tile again where there is none: the number of loads in
                 // flight stays the same on every path, so that no wait is longer than it has to be)
@@ -674,14 +665,15 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_attention_kernel(const estts
                 walk.locate(nx, nx != it);
                 load_k(nx);
                 if (drop) {
-                    if constexpr (!MASK) find_in();
+                    const uint32_t mine = rows_in >> (4 * g);
 #pragma unroll
                     for (int s = 0; s < HALVES; ++s)
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
-                            sc[s][j] = in[s][j] ? sc[s][j] : -INFINITY;
+                            const bool in = mine >> (16 * s + j) & 1;
+                            sc[s][j] = in ? sc[s][j] : -INFINITY;
 #pragma unroll
-                            for (int x = 0; x < VW; ++x) vr[s][j][x] = in[s][j] ? vr[s][j][x] : 0;       // (0 x NaN would be NaN)
+                            for (int x = 0; x < VW; ++x) vr[s][j][x] = in ? vr[s][j][x] : 0;       // (0 x NaN would be NaN)
                         }
                 }
                 // softmax step
@@ -777,6 +769,7 @@ __device__ __forceinline__ float row_sum(float v) {     // over the 16 lanes of 
 
 template <int DH, bool MASK, bool STREAM, int NQ, int NW>
 __global__ __launch_bounds__(NW * 64, 2) void paged_attention_few_kernel(const estts_paged_attention_args p, const int target) {
+    constexpr uint32_t ALL_ROWS = tile_halves(DH, 4) == 2 ? 0xFFFFFFFFu : 0xFFFFu;
     constexpr int HALVES = tile_halves(DH, 4), TILE = 16 * HALVES, NV = DH / 16, RUN = NV < 4 ? NV : 4;
     typedef __attribute__((ext_vector_type(RUN))) float run_t;
     __shared__ __attribute__((aligned(16))) float o_s[NW][NQ][DH];
@@ -805,7 +798,7 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_attention_few_kernel(const e
         const int lane_at = 4 * g * row_bytes + i * 4 * RUN;
 
         float kr[HALVES][4][NV], vr[HALVES][4][NV];
-        [[maybe_unused]] float mk[HALVES][4];
+        [[maybe_unused]] float mk;
         auto load = [&](const char* base, float (&r)[HALVES][4][NV], auto hint) {
 #pragma unroll
             for (int s = 0; s < HALVES; ++s)
@@ -824,14 +817,7 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_attention_few_kernel(const e
         auto load_k = [&]() { load(kbase, kr, std::false_type()); };
         auto load_v = [&]() { load(vbase, vr, std::bool_constant<STREAM>()); };
         auto load_mask = [&](int it) {
-            if constexpr (MASK) {
-                const float* mrow = p.key_mask + b * p.mask_sb;
-                const int r0 = begin + (it * NW + wave) * TILE + 4 * g;
-#pragma unroll
-                for (int s = 0; s < HALVES; ++s)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) mk[s][j] = mrow[min(r0 + 16 * s + j, end - 1) * p.mask_ss];
-            }
+            if constexpr (MASK) mk = p.key_mask[b * p.mask_sb + min(begin + (it * NW + wave) * TILE + lane % TILE, end - 1) * p.mask_ss];
         };
         float m[NQ], l[NQ], o[NQ][NV];
 #pragma unroll
@@ -866,29 +852,27 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_attention_few_kernel(const e
                             for (int e = 1; e < NV; ++e) t = fmaf(kr[s][j][e], qx[n][e], t);
                             sc[n][s][j] = row_sum(t);
                         }
-                bool in[HALVES][4], mine = true;
-#pragma unroll
-                for (int s = 0; s < HALVES; ++s)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        in[s][j] = ok_now[s] && r0 + 16 * s + 4 * g + j < end;
-                        if constexpr (MASK) in[s][j] = in[s][j] && mk[s][j] == 0.0f;
-                        mine = mine && in[s][j];
-                    }
-                const bool drop = MASK ? (bool)__any(!mine) : !all_in;
+                uint32_t rows_in = 0;
+                bool drop = !all_in;
+                if (MASK || drop) {
+                    rows_in = rows_that_count<HALVES>(r0, end, ok_now, MASK ? mk : 0.0f);
+                    drop = rows_in != ALL_ROWS;
+                }
                 const int nx = min(it + 1, n_mine - 1);
                 walk.locate(nx, nx != it);
                 load_k();
                 load_mask(nx);
                 if (drop) {
+                    const uint32_t mine = rows_in >> (4 * g);
 #pragma unroll
                     for (int s = 0; s < HALVES; ++s)
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
+                            const bool in = mine >> (16 * s + j) & 1;
 #pragma unroll
-                            for (int n = 0; n < NQ; ++n) sc[n][s][j] = in[s][j] ? sc[n][s][j] : -INFINITY;
+                            for (int n = 0; n < NQ; ++n) sc[n][s][j] = in ? sc[n][s][j] : -INFINITY;
 #pragma unroll
-                            for (int e = 0; e < NV; ++e) vr[s][j][e] = in[s][j] ? vr[s][j][e] : 0.0f;
+                            for (int e = 0; e < NV; ++e) vr[s][j][e] = in ? vr[s][j][e] : 0.0f;
                         }
                 }
 #pragma unroll
