@@ -794,7 +794,7 @@ def paged_attention(q, k_cache, v_cache, block_table, lengths, ctx, heads, key_m
     max_len = P * page if max_len is None else min(int(max_len), P * page)
     if max_len < 1:
         raise ValueError('paged_attention: max_len must be positive')
-    if heads < 1 or heads % Hk:
+    if heads < 1 or Hk < 1 or heads % Hk:
         raise ValueError(f'paged_attention: {heads} query heads do not divide over {Hk} key heads')
     width = heads * D
     ldq, ldo = _check_rows('paged_attention', q, 'q', B, width), _check_rows('paged_attention', ctx, 'ctx', B, width)

@@ -143,6 +143,12 @@ def test_paged_attention_checks_its_arguments(bad, error):
         ops.paged_attention(**f)
 
 
+def test_caches_without_heads_or_rows_are_refused():
+    for shape, error in (((32, 0, 16, 64), 'do not divide'), ((32, 4, 0, 64), 'max_len')):
+        with pytest.raises(ValueError, match=error):
+            ops.paged_attention(torch.zeros(4, 256), torch.zeros(shape), torch.zeros(shape), i32(4, 8), i32(4), torch.zeros(4, 256), 4)
+
+
 def test_pages_must_be_a_multiple_of_sixteen_rows():
     lib = _lib.load()
     for page in (1, 8, 15, 17, 40):
