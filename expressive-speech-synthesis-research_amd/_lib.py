@@ -307,9 +307,9 @@ def load():
 _host = None
 
 
-def load_host(scratch):
-    """The C module that issues the paged-decoding operators (csrc/hostops.c), set up with this library's entry points and torch's
-    device and stream queries; raise if it is not built.  scratch(nbytes, device): a tensor for one launch."""
+def load_host():
+    """The C++ module that issues the paged-decoding operators (csrc/hostops.cpp), set up with this library's entry points and torch's
+    allocator, device and stream queries; raise if it is not built."""
     global _host
     if _host is None:
         lib = load()
@@ -323,7 +323,8 @@ def load_host(scratch):
         spec.loader.exec_module(mod)
         at = [C.cast(getattr(lib, n), _vp).value for n in ('estts_page_plan', 'estts_page_write', 'estts_paged_attention', 'estts_page_plan_ws_bytes',
                                                            'estts_paged_attention_ws_bytes')]
-        mod.setup(*at, scratch, torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream, torch.int32, torch.float32, torch.bfloat16, torch.float16)
+        mod.setup(*at, torch._C._cuda_cudaCachingAllocator_raw_alloc, torch._C._cuda_cudaCachingAllocator_raw_delete, torch._C._cuda_getDevice,
+                  torch._C._cuda_getCurrentRawStream)
         _host = mod
     return _host
 

@@ -691,11 +691,11 @@ def _check_pages(what, k_cache, v_cache):
 
 
 def _issue():
-    """The C module that issues plain calls of the operators below, None while launches are recorded, traced or named: those, and whatever
+    """The C++ module that issues plain calls of the operators below, None while launches are recorded, traced or named: those, and whatever
     the module turns down, take the Python path behind it, which says what is wrong."""
     if _program is not None or _trace is not None or _debug_sync:
         return None
-    return _lib._host or _lib.load_host(_scratch)
+    return _lib._host or _lib.load_host()
 
 
 def new_paged_cache(n_pages, page, kv_heads, depth, dtype=torch.float32, device='cuda'):

@@ -655,7 +655,7 @@ def python_path(monkeypatch):
 
 @pytest.mark.parametrize('kind', sorted(TYPES))
 def test_the_c_module_and_the_python_path_issue_the_same_launches(monkeypatch, kind):
-    """A loop through csrc/hostops.c and one through the Python path: the same bits everywhere.  While the first runs the argument blocks of
+    """A loop through csrc/hostops.cpp and one through the Python path: the same bits everywhere.  While the first runs the argument blocks of
     the second are out of reach, so that it cannot have taken that path."""
     width, steps = Loop(kind).qkv.shape[1], 24
     plan = feeds(5, width, steps, 21)
@@ -732,3 +732,40 @@ def test_calls_the_c_module_leaves_to_python_work(monkeypatch):
     b = ops.paged_attention(q, *args, torch.empty(1, 64, device=DEV), 1, scale=1.0, max_len=16.0)
     python_path(monkeypatch)
     assert torch.equal(a, b) and torch.equal(a, ops.paged_attention(q, *args, torch.empty(1, 64, device=DEV), 1, scale=1.0))
+
+
+class Named(torch.Tensor):
+    pass
+
+
+def test_parameters_subclasses_and_large_offsets_are_taken_by_either_path():
+    kc, vc = cache_pair(40, 16, 2, 64, torch.float16)
+    g = torch.Generator().manual_seed(4)
+    for c in (kc, vc):
+        c.copy_(torch.randn(c.shape, generator=g))
+    q = torch.randn(2, 256, generator=g).to(DEV)
+    args = (kc, vc, torch.arange(40, dtype=torch.int32, device=DEV).view(2, 20), dev([300, 77]))
+    attend = lambda x, *a: ops.paged_attention(x, *(a or args), torch.empty(2, 256, device=DEV), 4)
+    want = attend(q)
+    assert torch.equal(want, attend(torch.nn.Parameter(q))) and torch.equal(want, attend(q.as_subclass(Named)))
+    assert torch.equal(want, attend(q, kc.as_subclass(Named), *args[1:]))
+
+
+def test_scratch_goes_back_to_the_allocator():
+    """Calls in two launches, good and bad ones, on two streams: what is allocated afterwards is what was before."""
+    kc, vc = cache_pair(600, 16, 2, 64, torch.bfloat16)
+    q, ctx = torch.randn(3, 256, device=DEV), torch.empty(3, 256, device=DEV)
+    table, lengths = torch.arange(600, dtype=torch.int32, device=DEV).view(3, 200), dev([3200, 1, 1700])
+    slots, free, n_free, new = (torch.empty(6000, dtype=torch.int32, device=DEV), torch.arange(600, dtype=torch.int32, device=DEV), dev([0]), dev([0, 0, 0]))
+    assert ops._lib.load().estts_paged_attention_ws_bytes(3, 4, 2, 64, 3200) > 0 and ops._lib.load().estts_page_plan_ws_bytes(3, 6000) > 0
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    for stream in (torch.cuda.current_stream(), torch.cuda.Stream()):
+        with torch.cuda.stream(stream):
+            for _ in range(20):
+                ops.paged_attention(q, kc, vc, table, lengths, ctx, 4)
+                ops.page_plan(lengths, new, table, free, n_free, 16, slots)
+                with pytest.raises(ops._lib.EsttsError):
+                    ops.page_plan(lengths, new, table, free, n_free, 24, slots)
+        torch.cuda.synchronize()
+    assert torch.cuda.memory_allocated() == before
