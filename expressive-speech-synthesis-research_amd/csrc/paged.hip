@@ -9,23 +9,43 @@ namespace {
 // ------------------------------------------------------------------------------------------------ page plan
 // Whole-number work on a few kilobytes, bound by latency: a launch, the lengths, the scans, the stack or the table, the maps.  One
 // workgroup scans the requests; the copies and the rows' places are then made by the same workgroup, or by a second launch
-// of as many as it takes where there are more than PLAN_ROWS rows (one workgroup for all: 64 prompts of 2047 rows at most 95 us, now 8.6;
-// 1000 requests that end, grow and arrive, 26000 rows, 84 us, now 14).  A step of 32 requests is one launch of 4.3 us, some 2 of which are
+// of as many as it takes where there are more than PLAN_ROWS rows (one workgroup for all: 64 prompts of 2047 rows at most 95 us, now 7.1;
+// 1000 requests that end, grow and arrive, 26000 rows, 84 us, now 10.6).  A step of 32 requests is one launch of 3.2 us, some 2 of which are
 // the launch itself.
 constexpr int PLAN_LDS = 4096;         // requests whose plan fits the LDS (four ints each); beyond that it lives in the caller's scratch
 
 __device__ __forceinline__ int pages_of(int rows, int page) { return (int)(((unsigned)rows + page - 1) / (unsigned)page); }
 
-// inclusive prefix sum over the workgroup's NT threads, and the total
+// A value from another lane, 0 where there is none: CTRL says which (row_shr 1, 2, 4, 8: that many lanes below in the row of 16; row_bcast 15, 31:
+// the last lane of the row, of the half wave before), ROWS which rows of 16 take it.
+template <int CTRL, int ROWS, typename V>
+__device__ __forceinline__ V from_lane(V v) {
+    if constexpr (sizeof(V) == 4) {
+        return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false);
+    } else {
+        const unsigned lo = __builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
+        const int hi = __builtin_amdgcn_update_dpp(0, (int)(v >> 32), CTRL, ROWS, 0xf, false);
+        return (V)(((unsigned long long)(unsigned)hi << 32) | lo);
+    }
+}
+
+// inclusive prefix sum over the wave: no LDS, six additions (with shuffles, which go through the LDS, a plan of 32 requests took 4.5 us
+// where it then took 3.7, one of 1000 13.9 and 12.7)
+template <typename V>
+__device__ __forceinline__ V wave_scan(V v) {
+    v += from_lane<0x111, 0xf>(v);
+    v += from_lane<0x112, 0xf>(v);
+    v += from_lane<0x114, 0xf>(v);
+    v += from_lane<0x118, 0xf>(v);
+    v += from_lane<0x142, 0xa>(v);
+    return v + from_lane<0x143, 0xc>(v);
+}
+
+// inclusive prefix sum over the workgroup's NT threads, and the total.  part: of this scan alone until every thread has passed another barrier.
 template <int NT, typename V>
 __device__ __forceinline__ V block_scan(V v, V* part, V& total) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const V up = __shfl_up(v, d);
-        if (lane >= d) v += up;
-    }
-    __syncthreads();                       // (the last scan's readers of part are done)
+    v = wave_scan(v);
     if (lane == 63) part[wave] = v;
     __syncthreads();
     V before = 0;
@@ -39,7 +59,7 @@ __device__ __forceinline__ V block_scan(V v, V* part, V& total) {
     return v + before;
 }
 
-// first b with end[b] > x (ends do not decrease); B if there is none
+// first b with end[b] > x (ends do not decrease); B if there is none.  (Three looks at a time, so half as many waits, were no faster.)
 __device__ __forceinline__ int first_past(const int* end, int B, int x) {
     int lo = 0, hi = B;
     while (lo < hi) {
@@ -51,7 +71,7 @@ __device__ __forceinline__ int first_past(const int* end, int B, int x) {
 
 // What is known of each request after the scans.  Up to PLAN_LDS requests it is held in the LDS.
 struct PagePlan {
-    const int* row_end;        // end of its rows in a packed map (at most T)
+    const int* row_end;        // end of its rows in a packed map (at most T); their number where the map is padded
     const int* back_end;       // pages given back up to and including it
     const int* page_end;       // pages granted up to and including it
     const int* len_of;         // its length, complemented where it gets no rows
@@ -62,6 +82,7 @@ constexpr int PLAN_HEAD = 4;   // scratch of a plan in two launches: height0, ba
 // The copies that a plan asks for, in any order and by any thread: every source is as the call found it.  Place e of the stack with the
 // given-back pages on it is free_pages[e] below height0, above it the page of an ended request; a row's page is in the table if the
 // request held it already, else on the stack.
+template <bool RUNS>
 __device__ __forceinline__ void carry_out(const estts_page_plan_args& p, const PagePlan& q, const int first, const int step) {
     auto given_back = [&](int g) {
         const int b = first_past(q.back_end, p.B, g);
@@ -69,36 +90,74 @@ __device__ __forceinline__ void carry_out(const estts_page_plan_args& p, const P
     };
     auto on_stack = [&](int e) { return e < q.height0 ? p.free_pages[e] : given_back(e - q.height0); };
     const int height = q.height0 + q.back;
-    for (int t = first; t < p.T; t += step) {
-        const int b = p.R ? t / p.R : first_past(q.row_end, p.B, t);
-        int slot = -1, pos = -1;
-        const int len = b < p.B ? q.len_of[b] : -1;
-        if (len >= 0) {
-            const int i = p.R ? t - b * p.R : t - (b ? q.row_end[b - 1] : 0);
-            if (!p.R || i < p.n_new[b]) {
-                pos = len + i;
-                const int j = pos / p.page, fresh = j - pages_of(len, p.page);
-                const int id = fresh < 0 ? p.block_table[b * p.ld_table + j] : on_stack(height - 1 - ((b ? q.page_end[b - 1] : 0) + fresh));
-                if (id >= 0 && id < p.n_pages) slot = id * p.page + (pos - j * p.page);
+    // rows, pages taken and pages given back one behind the other, so that threads without rows begin with the pages at once
+    const int rows = (p.T + 63) & ~63, work = rows + q.taken;           // (whole waves of rows)
+    for (int x = first; x < work; x += step) {
+        if (x >= rows) {
+            const int g = x - rows, b = first_past(q.page_end, p.B, g);
+            const int i = g - (b ? q.page_end[b - 1] : 0);
+            p.block_table[b * p.ld_table + pages_of(q.len_of[b], p.page) + i] = on_stack(height - 1 - g);
+        } else if (x < p.T) {
+            const int b = p.R ? x / p.R : first_past(q.row_end, p.B, x);
+            int slot = -1, pos = -1;
+            const int len = b < p.B ? q.len_of[b] : -1;
+            if (len >= 0) {
+                const int i = p.R ? x - b * p.R : x - (b ? q.row_end[b - 1] : 0);
+                if (!p.R || i < q.row_end[b]) {
+                    pos = len + i;
+                    const int j = pos / p.page, fresh = j - pages_of(len, p.page);
+                    const int id = fresh < 0 ? p.block_table[b * p.ld_table + j] : on_stack(height - 1 - ((b ? q.page_end[b - 1] : 0) + fresh));
+                    if (id >= 0 && id < p.n_pages) slot = id * p.page + (pos - j * p.page);
+                }
             }
+            p.slots[x] = slot;
+            if (p.positions) p.positions[x] = pos;
         }
-        p.slots[t] = slot;
-        if (p.positions) p.positions[t] = pos;
     }
-    for (int g = first; g < q.taken; g += step) {
-        const int b = first_past(q.page_end, p.B, g);
-        const int i = g - (b ? q.page_end[b - 1] : 0);
-        p.block_table[b * p.ld_table + pages_of(q.len_of[b], p.page) + i] = on_stack(height - 1 - g);
+    if (!RUNS || q.back <= 4 * step) {
+        const int behind = first - (int)((unsigned)work % (unsigned)step);
+#pragma unroll 1
+        for (int g = behind < 0 ? behind + step : behind; g < q.back; g += step) p.free_pages[q.height0 + g] = given_back(g);
+        return;
     }
-#pragma unroll 4
-    for (int g = first; g < q.back; g += step) p.free_pages[q.height0 + g] = given_back(g);
+    // Many pages for few threads: a run for each wave, in pieces of one request's pages (at most 64), four in flight; looking each page up
+    // by itself takes a thread 0.8 us a page (100 of 1000 requests of up to 4096 rows end: 17.3 us, like this 13.6).  Only in the kernel of
+    // 1024 threads: the longer code alone costs the others 0.1 to 0.4 us.
+    const int lane = first & 63, waves = step >> 6, per = (q.back + 64 * waves - 1) / (64 * waves) * 64;
+    int g = __builtin_amdgcn_readfirstlane(first >> 6) * per;
+    const int last = min(g + per, q.back);
+    if (g >= last) return;
+    int b = first_past(q.back_end, p.B, g);
+    while (g < last) {
+        int id[4], at[4], n[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            at[k] = g;
+            n[k] = 0;
+            if (g >= last) continue;
+            const int end = q.back_end[b], from = b ? q.back_end[b - 1] : 0;
+            n[k] = min(min(end, last) - g, 64);
+            if (lane < n[k]) id[k] = p.block_table[b * p.ld_table + (g - from) + lane];
+            g += n[k];
+            if (g < end || g >= last) continue;
+            uint64_t hit;                           // the next request that gives any back (there is one: g < back)
+            do {
+                const int x = b + 1 + lane;
+                hit = __ballot(x < p.B && q.back_end[min(x, p.B - 1)] > g);
+                b += hit ? __builtin_ctzll(hit) + 1 : 64;
+            } while (!hit);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (lane < n[k]) p.free_pages[q.height0 + at[k] + lane] = id[k];
+    }
 }
 
 // The scans, by one workgroup; then the copies, unless they are left to page_copy_kernel (split != 0; the plan goes to p.ws).
 template <int NT, bool LDS>
 __global__ __launch_bounds__(NT) void page_plan_kernel(const estts_page_plan_args p, const int split) {
-    __shared__ int part_i[NT / 64];
-    __shared__ long long part_l[NT / 64];
+    __shared__ int back_s[NT / 64], need_s[2][NT / 64];
+    __shared__ long long rows_s[NT / 64];
     __shared__ int taken_s, refused_s;
     __shared__ int plan_s[LDS ? 4 * PLAN_LDS : 1];
     const int tid = threadIdx.x;
@@ -109,7 +168,7 @@ __global__ __launch_bounds__(NT) void page_plan_kernel(const estts_page_plan_arg
 
     const int height0 = min(max(p.n_free[0], 0), p.n_pages);
     if (tid == 0) taken_s = refused_s = 0;
-    // rows before each request; pages of the requests that ended
+    // rows before each request; pages of the requests that ended (two scans a turn: the barrier of each lies between two uses of the other's sums)
     int back = 0;
     long long rows_before = 0;
     for (int b0 = 0; b0 < p.B; b0 += NT) {
@@ -117,13 +176,13 @@ __global__ __launch_bounds__(NT) void page_plan_kernel(const estts_page_plan_arg
         const int n = b < p.B ? p.n_new[b] : 0;
         const int len = b < p.B ? min(max(p.lengths[b], 0), cap) : 0;
         int back_total;
-        const int upto = back + block_scan<NT>(n < 0 ? pages_of(len, p.page) : 0, part_i, back_total);
+        const int upto = back + block_scan<NT>(n < 0 ? pages_of(len, p.page) : 0, back_s, back_total);
         long long rows_total;
-        const long long rows_upto = rows_before + block_scan<NT>((long long)max(n, 0), part_l, rows_total);
+        const long long rows_upto = rows_before + block_scan<NT>((long long)max(n, 0), rows_s, rows_total);
         if (b < p.B) {
             back_end[b] = upto;
             const bool inside = n <= 0 || (p.R ? n <= p.R : rows_upto <= p.T);
-            row_end[b] = (int)min(rows_upto, (long long)p.T);
+            row_end[b] = p.R ? max(n, 0) : (int)min(rows_upto, (long long)p.T);
             len_of[b] = inside ? len : ~len;
         }
         back += back_total;
@@ -133,14 +192,14 @@ __global__ __launch_bounds__(NT) void page_plan_kernel(const estts_page_plan_arg
     const int height = height0 + back;
     // grants
     int asked = 0;
-    for (int b0 = 0; b0 < p.B; b0 += NT) {
+    for (int b0 = 0, turn = 0; b0 < p.B; b0 += NT, turn ^= 1) {         // (two sets of sums in turn: one barrier lies between uses of the same)
         const int b = b0 + tid;
         const int n = b < p.B ? p.n_new[b] : 0;
         const int mark = b < p.B ? len_of[b] : 0, len = mark < 0 ? ~mark : mark;
         const bool fits = b < p.B && n >= 0 && mark >= 0 && len + (long long)n <= cap;
         const int need = fits ? pages_of(len + n, p.page) - pages_of(len, p.page) : 0;
         int need_total;
-        const int upto = asked + block_scan<NT>(need, part_i, need_total);
+        const int upto = asked + block_scan<NT>(need, need_s[turn], need_total);
         const bool granted = fits && (need == 0 || upto <= height);
         if (b < p.B) {
             page_end[b] = min(upto, height);        // (a request that is turned away ends no page below its own)
@@ -165,7 +224,7 @@ __global__ __launch_bounds__(NT) void page_plan_kernel(const estts_page_plan_arg
                 for (int k = 0; k < 4; ++k) p.ws[PLAN_HEAD + k * p.B + b] = plan[k * pitch + b];
         return;
     }
-    carry_out(p, {row_end, back_end, page_end, len_of, height0, back, taken}, tid, NT);
+    carry_out<NT == 1024>(p, {row_end, back_end, page_end, len_of, height0, back, taken}, tid, NT);
 }
 
 template <bool LDS>
@@ -180,7 +239,7 @@ __global__ __launch_bounds__(256) void page_copy_kernel(const estts_page_plan_ar
         __syncthreads();
         plan = plan_s;
     }
-    carry_out(p, {plan, plan + p.B, plan + 2 * (long)p.B, plan + 3 * (long)p.B, height0, back, taken}, blockIdx.x * 256 + threadIdx.x, gridDim.x * 256);
+    carry_out<false>(p, {plan, plan + p.B, plan + 2 * (long)p.B, plan + 3 * (long)p.B, height0, back, taken}, blockIdx.x * 256 + threadIdx.x, gridDim.x * 256);
 }
 
 // ------------------------------------------------------------------------------------------------ rows into the pages
@@ -1041,8 +1100,9 @@ extern "C" int estts_page_plan(const estts_page_plan_args* args, void* stream) {
     else if (a.B > 256 || (!split && a.T > 1024)) ESTTS_LAUNCH((page_plan_kernel<1024, true>), dim3(1), dim3(1024), 0, st, a, split);
     else ESTTS_LAUNCH((page_plan_kernel<256, true>), dim3(1), dim3(256), 0, st, a, split);
     if (split) {
-        const int wgs = (a.T + 255) / 256;
-        const dim3 grid(wgs < 1024 ? wgs : 1024);
+        // (threads enough for the rows, for the pages that they may take and for those that may come back)
+        const long wgs = ((long)a.T + a.T / a.page + a.B + a.n_pages + 255) / 256;
+        const dim3 grid((unsigned)(wgs < 1024 ? wgs : 1024));
         if (a.B > PLAN_LDS) ESTTS_LAUNCH(page_copy_kernel<false>, grid, dim3(256), 0, st, a);
         else ESTTS_LAUNCH(page_copy_kernel<true>, grid, dim3(256), 0, st, a);
     }

@@ -150,6 +150,32 @@ def test_page_plan_of_long_packed_prompts(B, T):
         assert run_plan(lengths, new, table, free, n, page, T=T, in_place=in_place) == want
 
 
+@pytest.mark.parametrize('B,longest,ends,size', [(300, 3000, lambda b: b % 3 == 1, dict(R=1)), (64, 5000, lambda b: b % 2 == 0, dict(T=1500)),
+                                                 (1200, 160, lambda b: b % 7 != 0, dict(R=2)), (1000, 50000, lambda b: b in (3, 400, 401, 999), dict(T=1000)),
+                                                 (2, 99999, lambda b: b == 0, dict(R=1000)), (5000, 100, lambda b: b % 2 == 1, dict(T=4000))])
+@pytest.mark.parametrize('twice', [False, True])
+def test_page_plan_takes_back_many_pages(B, longest, ends, size, twice):
+    """More pages come back than the one workgroup has threads; twice: as many again as there are, where it has to stop."""
+    page, g = 16, torch.Generator().manual_seed(B)
+    lengths = [int(torch.randint(0, longest + 1 if ends(b) else 41, (1,), generator=g)) for b in range(B)]
+    P = -(-longest // page) + 1
+    used = [-(-n // page) for n in lengths]
+    n = sum(used) + 3
+    ids, table, at = torch.randperm(n, generator=g).tolist(), [], 0
+    for u in used:
+        table.append(ids[at:at + u] + [-5] * (P - u))
+        at += u
+    back = sum(u for b, u in enumerate(used) if ends(b))
+    assert back > 4096
+    free, n_free = ids[at:] + [-9] * at, n - at
+    if twice:
+        n_free = n - back // 2                       # (some of what is on the stack is held as well)
+        free = (ids[::-1])[:n_free] + [-9] * (n - n_free)
+    new = [-1 if ends(b) else b % 3 for b in range(B)]
+    want = plan_oracle(lengths, new, table, free, n_free, page, **size)
+    assert run_plan(lengths, new, table, free, n_free, page, **size) == want
+
+
 def test_page_plan_keeps_every_page_exactly_once():
     """A serving loop with requests that come, grow, wait and end: no page is lost or held twice, in place over many steps."""
     B, P, page, n = 70, 6, 16, 150
