@@ -362,13 +362,13 @@ __device__ __forceinline__ int request_rows(const estts_paged_attention_args& p,
     return min(min(max(p.lengths[b], 0), p.P * p.page), p.max_len);
 }
 
-// How the rows are dealt out.  target == 0: a workgroup has a whole request (and a key head's queries).  Else all rows of all requests,
+// How the rows are dealt out.  SPLIT false: a workgroup has a whole request (and a key head's queries).  Else all rows of all requests,
 // in units of UNIT, are one line that is cut into equal parts, so that long and short requests keep the chip equally busy and no part
 // is last; the host knows no lengths, the parts follow from them on the GPU.  A part holds whole requests, the end of one that began in
 // an earlier part and the beginning of one that goes on in a later part: two places of scratch a part, 2k and 2k + 1, hold the latter two.
 struct PagedSegment { int b, begin, end, place; bool whole; };      // rows [begin, end) of request b; place: of the scratch, unless whole
 
-template <int NT, int UNIT>
+template <int NT, int UNIT, bool SPLIT>
 struct PagedPart {
     int k, parts, b, off, left, total, at;      // requests from b on, of b the units from off on, left units in all; at: place of unit off of b in the line
 
@@ -376,7 +376,7 @@ struct PagedPart {
 
     __device__ __forceinline__ bool find(const estts_paged_attention_args& p, int part, int target) {
         int first = part, from = 0, to = 0, skip = 0, all = 1, n_parts = 1;
-        if (target) {
+        if constexpr (SPLIT) {
             __shared__ int scan_s[NT / 64], found_s[2];
             const int per = (p.B + NT - 1) / NT, b0 = threadIdx.x * per, b1 = min(b0 + per, p.B);
             int mine = 0;                       // (the sum over all is at most 2^30: the caller keeps B * max_len below 2^36)
@@ -406,16 +406,16 @@ struct PagedPart {
         off = __builtin_amdgcn_readfirstlane(skip);
         left = to - from;
         at = from;
-        return part < (target ? n_parts : p.B);
+        return part < (SPLIT ? n_parts : p.B);
     }
 
     // the next rows to do; items (of the first key head's workgroups): where the join finds request b
-    __device__ __forceinline__ PagedSegment next(const estts_paged_attention_args& p, int target, int2* items) {
+    __device__ __forceinline__ PagedSegment next(const estts_paged_attention_args& p, int2* items) {
         const int rows = __builtin_amdgcn_readfirstlane(request_rows(p, b));
-        const int n = units_of(rows), take = target ? min(n - off, left) : n;
-        const PagedSegment s = {b, off * UNIT, min(rows, (off + take) * UNIT), 2 * k + (off == 0), take == n};
+        const int n = units_of(rows), take = SPLIT ? min(n - off, left) : n;
+        const PagedSegment s = {b, off * UNIT, min(rows, (off + take) * UNIT), 2 * k + (off == 0), !SPLIT || take == n};
         // unit x of the line is in part floor(((x + 1) parts - 1) / total)
-        if (target && off == 0 && items) items[b] = make_int2(k, take == n ? 1 : (int)((((long)at + n) * parts - 1) / total) - k + 1);
+        if (SPLIT && off == 0 && items) items[b] = make_int2(k, take == n ? 1 : (int)((((long)at + n) * parts - 1) / total) - k + 1);
         left -= take;
         at += take;
         off = 0;
@@ -543,7 +543,9 @@ __device__ __forceinline__ void join_waves(const estts_paged_attention_args& p, 
     }
 }
 
-template <typename T, int DH, bool MASK, bool STREAM, int NW>
+// SPLIT: the rows are cut into `target` parts.  (A kernel for each: the code of the cutting alone, not run, cost a short request 0.4 to 0.7 us,
+// one of 100 rows float32 4.2 / 3.6.)
+template <typename T, int DH, bool MASK, bool STREAM, bool SPLIT, int NW>
 __global__ __launch_bounds__(NW * 64, 2) void paged_attention_kernel(const estts_paged_attention_args p, const int target) {
     constexpr bool F32 = sizeof(T) == 4;
     constexpr int HALVES = tile_halves(DH, sizeof(T));
@@ -559,10 +561,10 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_attention_kernel(const estts
     const PagedUnit<16> u(p);
     const int heads = u.heads, h0 = u.h0;
     const PagedScratch ws(p.ws, target, p.H, DH);
-    PagedPart<NW * 64, TILE * NW> part;
+    PagedPart<NW * 64, TILE * NW, SPLIT> part;
     if (!part.find(p, u.part, target)) return;
     do {
-        const PagedSegment seg = part.next(p, target, h0 == 0 && threadIdx.x == 0 ? ws.items : nullptr);
+        const PagedSegment seg = part.next(p, h0 == 0 && threadIdx.x == 0 ? ws.items : nullptr);
         const int b = seg.b, begin = seg.begin, end = seg.end;
         PageWalk<HALVES, NW> walk(p, b, begin, wave, sizeof(T));
 
@@ -806,8 +808,8 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_attention_kernel(const estts
         }
         __syncthreads();
         join_waves<NW, 16, DH>(p, u, seg, ws, o_s, m_s, l_s);
-        if (part.left > 0) __syncthreads();         // (before the next segment's shares)
-    } while (part.left > 0);
+        if (SPLIT && part.left > 0) __syncthreads();         // (before the next segment's shares)
+    } while (SPLIT && part.left > 0);
 }
 
 // The same for float32 pages and a key head that only one or two query heads read (NQ): most columns of a matrix tile would be empty
@@ -826,7 +828,7 @@ __device__ __forceinline__ float row_sum(float v) {     // over the 16 lanes of 
     return v;
 }
 
-template <int DH, bool MASK, bool STREAM, int NQ, int NW>
+template <int DH, bool MASK, bool STREAM, bool SPLIT, int NQ, int NW>
 __global__ __launch_bounds__(NW * 64, 2) void paged_attention_few_kernel(const estts_paged_attention_args p, const int target) {
     constexpr uint32_t ALL_ROWS = tile_halves(DH, 4) == 2 ? 0xFFFFFFFFu : 0xFFFFu;
     constexpr int HALVES = tile_halves(DH, 4), TILE = 16 * HALVES, NV = DH / 16, RUN = NV < 4 ? NV : 4;
@@ -837,10 +839,10 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_attention_few_kernel(const e
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const PagedUnit<NQ> u(p);
     const PagedScratch ws(p.ws, target, p.H, DH);
-    PagedPart<NW * 64, TILE * NW> part;
+    PagedPart<NW * 64, TILE * NW, SPLIT> part;
     if (!part.find(p, u.part, target)) return;
     do {
-        const PagedSegment seg = part.next(p, target, u.h0 == 0 && threadIdx.x == 0 ? ws.items : nullptr);
+        const PagedSegment seg = part.next(p, u.h0 == 0 && threadIdx.x == 0 ? ws.items : nullptr);
         const int b = seg.b, begin = seg.begin, end = seg.end;
         PageWalk<HALVES, NW> walk(p, b, begin, wave, 4);
         const float qs = p.scale * 1.4426950408889634f;
@@ -977,8 +979,8 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_attention_few_kernel(const e
         }
         __syncthreads();
         join_waves<NW, NQ, DH>(p, u, seg, ws, o_s, m_s, l_s);
-        if (part.left > 0) __syncthreads();         // (before the next segment's shares)
-    } while (part.left > 0);
+        if (SPLIT && part.left > 0) __syncthreads();         // (before the next segment's shares)
+    } while (SPLIT && part.left > 0);
 }
 
 // The parts of a request meet: one workgroup per (query head, request).  Each of its eight half-waves takes every eighth part, four at a
@@ -1152,32 +1154,38 @@ extern "C" int64_t estts_paged_attention_ws_bytes(int32_t B, int32_t H, int32_t 
     return target ? PagedScratch::bytes(target, H, depth, B) : 0;
 }
 
-template <typename T, int DH, bool MASK, bool STREAM>
+template <typename T, int DH, bool MASK, bool STREAM, bool SPLIT>
 static void launch_paged_attention(const estts_paged_attention_args& a, int target, hipStream_t stream) {
     const int group = a.H / a.kv_heads, n_group = (group + 15) / 16;
     const int units = (target ? target : a.B) * a.kv_heads;
     const dim3 grid(n_group > 1 ? (units + 7) / 8 * 8 * n_group : units), block(ATT_WAVES * 64);
     if constexpr (sizeof(T) == 4) {
         if (group == 1) {
-            ESTTS_LAUNCH((paged_attention_few_kernel<DH, MASK, STREAM, 1, ATT_WAVES>), grid, block, 0, stream, a, target);
+            ESTTS_LAUNCH((paged_attention_few_kernel<DH, MASK, STREAM, SPLIT, 1, ATT_WAVES>), grid, block, 0, stream, a, target);
             return;
         }
         if (group <= FEW_QUERIES) {
-            ESTTS_LAUNCH((paged_attention_few_kernel<DH, MASK, STREAM, FEW_QUERIES, ATT_WAVES>), grid, block, 0, stream, a, target);
+            ESTTS_LAUNCH((paged_attention_few_kernel<DH, MASK, STREAM, SPLIT, FEW_QUERIES, ATT_WAVES>), grid, block, 0, stream, a, target);
             return;
         }
     }
-    ESTTS_LAUNCH((paged_attention_kernel<T, DH, MASK, STREAM, ATT_WAVES>), grid, block, 0, stream, a, target);
+    ESTTS_LAUNCH((paged_attention_kernel<T, DH, MASK, STREAM, SPLIT, ATT_WAVES>), grid, block, 0, stream, a, target);
+}
+
+template <typename T, int DH, bool SPLIT>
+static void launch_paged_attention(const estts_paged_attention_args& a, int target, hipStream_t stream) {
+    const bool many = stream_rows(a);
+    if (a.key_mask && many) launch_paged_attention<T, DH, true, true, SPLIT>(a, target, stream);
+    else if (a.key_mask) launch_paged_attention<T, DH, true, false, SPLIT>(a, target, stream);
+    else if (many) launch_paged_attention<T, DH, false, true, SPLIT>(a, target, stream);
+    else launch_paged_attention<T, DH, false, false, SPLIT>(a, target, stream);
+    if (SPLIT) ESTTS_LAUNCH(paged_join_kernel<DH>, dim3(a.H, a.B), dim3(256), 0, stream, a, target);
 }
 
 template <typename T, int DH>
 static void launch_paged_attention(const estts_paged_attention_args& a, int target, hipStream_t stream) {
-    const bool many = stream_rows(a);
-    if (a.key_mask && many) launch_paged_attention<T, DH, true, true>(a, target, stream);
-    else if (a.key_mask) launch_paged_attention<T, DH, true, false>(a, target, stream);
-    else if (many) launch_paged_attention<T, DH, false, true>(a, target, stream);
-    else launch_paged_attention<T, DH, false, false>(a, target, stream);
-    if (target) ESTTS_LAUNCH(paged_join_kernel<DH>, dim3(a.H, a.B), dim3(256), 0, stream, a, target);
+    if (target) launch_paged_attention<T, DH, true>(a, target, stream);
+    else launch_paged_attention<T, DH, false>(a, target, stream);
 }
 
 template <typename T>
