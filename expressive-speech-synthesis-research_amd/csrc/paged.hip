@@ -82,7 +82,7 @@ constexpr int PLAN_HEAD = 4;   // scratch of a plan in two launches: height0, ba
 // The copies that a plan asks for, in any order and by any thread: every source is as the call found it.  Place e of the stack with the
 // given-back pages on it is free_pages[e] below height0, above it the page of an ended request; a row's page is in the table if the
 // request held it already, else on the stack.
-template <bool RUNS>
+template <bool PADDED, bool RUNS>
 __device__ __forceinline__ void carry_out(const estts_page_plan_args& p, const PagePlan& q, const int first, const int step) {
     auto given_back = [&](int g) {
         const int b = first_past(q.back_end, p.B, g);
@@ -98,14 +98,14 @@ __device__ __forceinline__ void carry_out(const estts_page_plan_args& p, const P
             const int i = g - (b ? q.page_end[b - 1] : 0);
             p.block_table[b * p.ld_table + pages_of(q.len_of[b], p.page) + i] = on_stack(height - 1 - g);
         } else if (x < p.T) {
-            const int b = p.R ? x / p.R : first_past(q.row_end, p.B, x);
+            const int b = PADDED ? (int)((unsigned)x / (unsigned)p.R) : first_past(q.row_end, p.B, x);
             int slot = -1, pos = -1;
             const int len = b < p.B ? q.len_of[b] : -1;
             if (len >= 0) {
-                const int i = p.R ? x - b * p.R : x - (b ? q.row_end[b - 1] : 0);
-                if (!p.R || i < q.row_end[b]) {
+                const int i = PADDED ? x - b * p.R : x - (b ? q.row_end[b - 1] : 0);
+                if (!PADDED || i < q.row_end[b]) {
                     pos = len + i;
-                    const int j = pos / p.page, fresh = j - pages_of(len, p.page);
+                    const int j = (int)((unsigned)pos / (unsigned)p.page), fresh = j - pages_of(len, p.page);
                     const int id = fresh < 0 ? p.block_table[b * p.ld_table + j] : on_stack(height - 1 - ((b ? q.page_end[b - 1] : 0) + fresh));
                     if (id >= 0 && id < p.n_pages) slot = id * p.page + (pos - j * p.page);
                 }
@@ -153,18 +153,19 @@ __device__ __forceinline__ void carry_out(const estts_page_plan_args& p, const P
     }
 }
 
-// The scans, by one workgroup; then the copies, unless they are left to page_copy_kernel (split != 0; the plan goes to p.ws).
-template <int NT, bool LDS>
-__global__ __launch_bounds__(NT) void page_plan_kernel(const estts_page_plan_args p, const int split) {
+// The scans, by one workgroup; then the copies, unless they are left to page_copy_kernel (SPLIT; the plan goes to p.ws).
+template <int NT, bool LDS, bool PADDED, bool SPLIT>
+__global__ __launch_bounds__(NT) void page_plan_kernel(const estts_page_plan_args p) {
     __shared__ int back_s[NT / 64], need_s[2][NT / 64];
     __shared__ long long rows_s[NT / 64];
     __shared__ int taken_s, refused_s;
-    __shared__ int plan_s[LDS ? 4 * PLAN_LDS : 1];
+    __shared__ int plan_s[!LDS ? 1 : SPLIT ? PLAN_LDS : 4 * PLAN_LDS];
     const int tid = threadIdx.x;
     const int cap = p.P * p.page;
-    const long pitch = LDS ? PLAN_LDS : p.B;
-    int* const plan = LDS ? plan_s : p.ws + PLAN_HEAD;
+    const long pitch = LDS && !SPLIT ? PLAN_LDS : p.B;
+    int* const plan = LDS && !SPLIT ? plan_s : p.ws + PLAN_HEAD;
     int *const row_end = plan, *const back_end = plan + pitch, *const page_end = plan + 2 * pitch, *const len_of = plan + 3 * pitch;
+    int* const mark_of = LDS && SPLIT ? plan_s : len_of;        // (what a thread reads again itself)
 
     const int height0 = min(max(p.n_free[0], 0), p.n_pages);
     if (tid == 0) taken_s = refused_s = 0;
@@ -177,13 +178,14 @@ __global__ __launch_bounds__(NT) void page_plan_kernel(const estts_page_plan_arg
         const int len = b < p.B ? min(max(p.lengths[b], 0), cap) : 0;
         int back_total;
         const int upto = back + block_scan<NT>(n < 0 ? pages_of(len, p.page) : 0, back_s, back_total);
-        long long rows_total;
-        const long long rows_upto = rows_before + block_scan<NT>((long long)max(n, 0), rows_s, rows_total);
+        long long rows_total = 0, rows_upto = 0;
+        if constexpr (PADDED) { if (b0 + NT < p.B) __syncthreads(); }       // (for back_s)
+        else rows_upto = rows_before + block_scan<NT>((long long)max(n, 0), rows_s, rows_total);
         if (b < p.B) {
             back_end[b] = upto;
-            const bool inside = n <= 0 || (p.R ? n <= p.R : rows_upto <= p.T);
-            row_end[b] = p.R ? max(n, 0) : (int)min(rows_upto, (long long)p.T);
-            len_of[b] = inside ? len : ~len;
+            const bool inside = n <= 0 || (PADDED ? n <= p.R : rows_upto <= p.T);
+            row_end[b] = PADDED ? max(n, 0) : (int)min(rows_upto, (long long)p.T);
+            mark_of[b] = inside ? len : ~len;
         }
         back += back_total;
         rows_before += rows_total;
@@ -195,7 +197,7 @@ __global__ __launch_bounds__(NT) void page_plan_kernel(const estts_page_plan_arg
     for (int b0 = 0, turn = 0; b0 < p.B; b0 += NT, turn ^= 1) {         // (two sets of sums in turn: one barrier lies between uses of the same)
         const int b = b0 + tid;
         const int n = b < p.B ? p.n_new[b] : 0;
-        const int mark = b < p.B ? len_of[b] : 0, len = mark < 0 ? ~mark : mark;
+        const int mark = b < p.B ? mark_of[b] : 0, len = mark < 0 ? ~mark : mark;
         const bool fits = b < p.B && n >= 0 && mark >= 0 && len + (long long)n <= cap;
         const int need = fits ? pages_of(len + n, p.page) - pages_of(len, p.page) : 0;
         int need_total;
@@ -216,18 +218,14 @@ __global__ __launch_bounds__(NT) void page_plan_kernel(const estts_page_plan_arg
         p.n_free_out[0] = height - taken;
         if (p.refused) p.refused[0] = refused_s;
     }
-    if (split) {
+    if constexpr (SPLIT) {
         if (tid == 0) { p.ws[0] = height0; p.ws[1] = back; p.ws[2] = taken; }
-        if (LDS)
-            for (int b = tid; b < p.B; b += NT)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) p.ws[PLAN_HEAD + k * p.B + b] = plan[k * pitch + b];
-        return;
+    } else {
+        carry_out<PADDED, NT == 1024>(p, {row_end, back_end, page_end, len_of, height0, back, taken}, tid, NT);
     }
-    carry_out<NT == 1024>(p, {row_end, back_end, page_end, len_of, height0, back, taken}, tid, NT);
 }
 
-template <bool LDS>
+template <bool LDS, bool PADDED>
 __global__ __launch_bounds__(256) void page_copy_kernel(const estts_page_plan_args p) {
     __shared__ __attribute__((aligned(16))) int plan_s[LDS ? 4 * PLAN_LDS : 4];
     const int* plan = p.ws + PLAN_HEAD;
@@ -239,7 +237,7 @@ __global__ __launch_bounds__(256) void page_copy_kernel(const estts_page_plan_ar
         __syncthreads();
         plan = plan_s;
     }
-    carry_out<false>(p, {plan, plan + p.B, plan + 2 * (long)p.B, plan + 3 * (long)p.B, height0, back, taken}, blockIdx.x * 256 + threadIdx.x, gridDim.x * 256);
+    carry_out<PADDED, false>(p, {plan, plan + p.B, plan + 2 * (long)p.B, plan + 3 * (long)p.B, height0, back, taken}, blockIdx.x * 256 + threadIdx.x, gridDim.x * 256);
 }
 
 // ------------------------------------------------------------------------------------------------ rows into the pages
@@ -1082,6 +1080,24 @@ extern "C" int64_t estts_page_plan_ws_bytes(int32_t B, int32_t T) {
     return B > PLAN_LDS || T > PLAN_ROWS ? 4 * (PLAN_HEAD + 4 * (int64_t)B) : 0;
 }
 
+template <bool PADDED, bool SPLIT>
+static void launch_page_scans(const estts_page_plan_args& a, hipStream_t st) {
+    if (a.B > PLAN_LDS) ESTTS_LAUNCH((page_plan_kernel<1024, false, PADDED, SPLIT>), dim3(1), dim3(1024), 0, st, a);
+    else if (a.B > 256 || (!SPLIT && a.T > 1024)) ESTTS_LAUNCH((page_plan_kernel<1024, true, PADDED, SPLIT>), dim3(1), dim3(1024), 0, st, a);
+    else ESTTS_LAUNCH((page_plan_kernel<256, true, PADDED, SPLIT>), dim3(1), dim3(256), 0, st, a);
+}
+
+template <bool PADDED>
+static void launch_page_plan(const estts_page_plan_args& a, hipStream_t st) {
+    if (a.T <= PLAN_ROWS) return launch_page_scans<PADDED, false>(a, st);
+    launch_page_scans<PADDED, true>(a, st);
+    // (threads enough for the rows, for the pages that they may take and for those that may come back)
+    const long wgs = ((long)a.T + a.T / a.page + a.B + a.n_pages + 255) / 256;
+    const dim3 grid((unsigned)(wgs < 1024 ? wgs : 1024));
+    if (a.B > PLAN_LDS) ESTTS_LAUNCH((page_copy_kernel<false, PADDED>), grid, dim3(256), 0, st, a);
+    else ESTTS_LAUNCH((page_copy_kernel<true, PADDED>), grid, dim3(256), 0, st, a);
+}
+
 extern "C" int estts_page_plan(const estts_page_plan_args* args, void* stream) {
     ESTTS_CHECK_ARG(args != nullptr, "estts_page_plan: null args");
     const estts_page_plan_args& a = *args;
@@ -1096,18 +1112,8 @@ extern "C" int estts_page_plan(const estts_page_plan_args* args, void* stream) {
     const int64_t need = estts_page_plan_ws_bytes(a.B, a.T);
     ESTTS_CHECK_ARG(need == 0 || (a.ws && a.ws_bytes >= need && !(reinterpret_cast<uintptr_t>(a.ws) & 15)),
                     "estts_page_plan: this call needs %ld bytes of scratch, 16-byte aligned (given: %ld)", (long)need, (long)a.ws_bytes);
-    const hipStream_t st = (hipStream_t)stream;
-    const int split = a.T > PLAN_ROWS;
-    if (a.B > PLAN_LDS) ESTTS_LAUNCH((page_plan_kernel<1024, false>), dim3(1), dim3(1024), 0, st, a, split);
-    else if (a.B > 256 || (!split && a.T > 1024)) ESTTS_LAUNCH((page_plan_kernel<1024, true>), dim3(1), dim3(1024), 0, st, a, split);
-    else ESTTS_LAUNCH((page_plan_kernel<256, true>), dim3(1), dim3(256), 0, st, a, split);
-    if (split) {
-        // (threads enough for the rows, for the pages that they may take and for those that may come back)
-        const long wgs = ((long)a.T + a.T / a.page + a.B + a.n_pages + 255) / 256;
-        const dim3 grid((unsigned)(wgs < 1024 ? wgs : 1024));
-        if (a.B > PLAN_LDS) ESTTS_LAUNCH(page_copy_kernel<false>, grid, dim3(256), 0, st, a);
-        else ESTTS_LAUNCH(page_copy_kernel<true>, grid, dim3(256), 0, st, a);
-    }
+    if (a.R) launch_page_plan<true>(a, (hipStream_t)stream);
+    else launch_page_plan<false>(a, (hipStream_t)stream);
     ESTTS_CHECK_LAUNCH("estts_page_plan");
     return 0;
 }
