@@ -620,7 +620,7 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_attention_kernel(const estts
         [[maybe_unused]] float mk;                          // mask of row lane % TILE of the tile
         const int k_lane = i * row_bytes + 16 * g;
         const int v_lane = 4 * g * row_bytes + i * VB;
-        const int half_bytes = 15 * row_bytes + DH * (int)sizeof(T);
+        int half_bytes = 15 * row_bytes + DH * (int)sizeof(T);         // (0 behind the last tile: such loads reach no memory)
         auto load_k = [&](int it) {
 #pragma unroll
             for (int s = 0; s < HALVES; ++s) {
@@ -718,10 +718,11 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_attention_kernel(const estts
                     rows_in = rows_that_count<HALVES>(r0, end, ok_now, MASK ? mk : 0.0f);
                     drop = rows_in != ALL_ROWS;
                 }
-                // the next tile's keys, into the registers just read (the last tile again where there is none: the number of loads in
-                // flight stays the same on every path, so that no wait is longer than it has to be)
+                // the next tile's keys, into the registers just read (loads of nothing where there is none: the number of loads in flight
+                // stays the same on every path, so that no wait is longer than it has to be)
                 const int nx = min(it + 1, n_mine - 1);
                 walk.locate(nx, nx != it);
+                if (nx == it) half_bytes = 0;
                 load_k(nx);
                 if (drop) {
                     const uint32_t mine = rows_in >> (4 * g);
@@ -854,7 +855,7 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_attention_few_kernel(const e
         const char* kbase = static_cast<const char*>(p.k_cache) + u.hk * p.s_head * 4;
         const char* vbase = static_cast<const char*>(p.v_cache) + u.hk * p.s_head * 4;
         const int row_bytes = (int)(p.s_row * 4);
-        const int lane_at = 4 * g * row_bytes + i * 4 * RUN;
+        int lane_at = 4 * g * row_bytes + i * 4 * RUN;      // (0 behind the last tile: one line for the whole wave)
 
         float kr[HALVES][4][NV], vr[HALVES][4][NV];
         [[maybe_unused]] float mk;
@@ -919,6 +920,7 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_attention_few_kernel(const e
                 }
                 const int nx = min(it + 1, n_mine - 1);
                 walk.locate(nx, nx != it);
+                if (nx == it) lane_at = 0;
                 load_k();
                 load_mask(nx);
                 if (drop) {
