@@ -302,7 +302,10 @@ __global__ __launch_bounds__(256) void page_write_kernel(const estts_page_write_
 
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
 
-constexpr int ATT_WAVES = 4;           // waves of a workgroup (8: 61 ragged requests 92.8 -> 98.4 us, 8 of 1000 rows 14.4 -> 15.8)
+// Waves of a workgroup: four; eight for whole requests on the vector ALU, whose arithmetic they spread (4 heads of 64, float32, four / eight: one
+// request of 600 rows 5.5 / 5.1 us, of 1000 7.1 / 6.7, 64 ragged ones of 600 9.6 / 9.3, one of 100 3.3 / 3.4; on the matrix cores, 32 heads on 8 of
+// 128, bfloat16, one of 1000 12.3 / 12.7, 128 ragged ones of 1000 56.2 / 58.3; cut, 61 ragged ones 89.4 / 90.3).
+constexpr int ATT_WAVES = 4, FEW_WAVES = 8;
 constexpr int FEW_QUERIES = 2;         // query heads per key head up to which float32 pages take the vector ALU
 
 // 16-row halves of a wave's tile
@@ -1168,12 +1171,13 @@ static void launch_paged_attention(const estts_paged_attention_args& a, int targ
     const int units = (target ? target : a.B) * a.kv_heads;
     const dim3 grid(n_group > 1 ? (units + 7) / 8 * 8 * n_group : units), block(ATT_WAVES * 64);
     if constexpr (sizeof(T) == 4) {
+        constexpr int NW = SPLIT ? ATT_WAVES : FEW_WAVES;
         if (group == 1) {
-            ESTTS_LAUNCH((paged_attention_few_kernel<DH, MASK, STREAM, SPLIT, 1, ATT_WAVES>), grid, block, 0, stream, a, target);
+            ESTTS_LAUNCH((paged_attention_few_kernel<DH, MASK, STREAM, SPLIT, 1, NW>), grid, dim3(NW * 64), 0, stream, a, target);
             return;
         }
         if (group <= FEW_QUERIES) {
-            ESTTS_LAUNCH((paged_attention_few_kernel<DH, MASK, STREAM, SPLIT, FEW_QUERIES, ATT_WAVES>), grid, block, 0, stream, a, target);
+            ESTTS_LAUNCH((paged_attention_few_kernel<DH, MASK, STREAM, SPLIT, FEW_QUERIES, NW>), grid, dim3(NW * 64), 0, stream, a, target);
             return;
         }
     }

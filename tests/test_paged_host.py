@@ -215,7 +215,7 @@ def test_parts_cover_every_row_once_and_the_join_finds_them(lengths, target, uni
     assert max(sizes) - min(sizes) <= 1
 
 
-@pytest.mark.parametrize('halves,waves', [(1, 4), (2, 4)])
+@pytest.mark.parametrize('halves,waves', [(1, 4), (2, 4), (1, 8), (2, 8)])
 @pytest.mark.parametrize('page', [16, 48, 64])
 @pytest.mark.parametrize('P,max_len,begin,end', [(1, 16, 0, 1), (3, 40, 0, 40), (70, 1000, 0, 1000), (70, 1111, 512, 1111), (700, 9000, 4096, 9000)])
 def test_page_walk_stays_inside_table_and_pages(halves, waves, page, P, max_len, begin, end):
