@@ -219,7 +219,7 @@ SIGNATURES = {
     'estts_page_plan_ws_bytes': (_i64, [_i32, _i32]),
     'estts_page_write': (_i32, [C.POINTER(PageWriteArgs), _vp]),
     'estts_paged_attention': (_i32, [C.POINTER(PagedAttentionArgs), _vp]),
-    'estts_paged_attention_ws_bytes': (_i64, [_i32, _i32, _i32, _i32, _i32]),
+    'estts_paged_attention_ws_bytes': (_i64, [_i32, _i32, _i32, _i32, _i32, _i32]),
     'estts_masked_mae': (_i32, [_vp, _i32, _vp, _i32, _vp, _i32, _i32, _vp]),
     'estts_wavernn_prep': (_i32, [C.POINTER(WavernnPrepArgs), _vp]),
     'estts_gru_gates': (_i32, [_vp, _i32, _vp, _i32, _vp, _i32, _vp, _i32, _vp, _i32, _i32, _i32, _vp]),

@@ -23,7 +23,7 @@ struct {
     int (*write)(const estts_page_write_args*, void*);
     int (*attention)(const estts_paged_attention_args*, void*);
     int64_t (*plan_ws)(int32_t, int32_t);
-    int64_t (*attention_ws)(int32_t, int32_t, int32_t, int32_t, int32_t);
+    int64_t (*attention_ws)(int32_t, int32_t, int32_t, int32_t, int32_t, int32_t);
     PyObject *alloc, *free, *get_device, *get_stream;
 } host;
 
@@ -233,7 +233,7 @@ bool paged_attention(PyObject* const* a, Py_ssize_t n) {
     w.s_page = kc.s[0]; w.s_head = kc.s[1]; w.s_row = kc.s[2];
     w.B = (int32_t)B; w.H = (int32_t)heads; w.n_pages = (int32_t)kc.n[0]; w.kv_heads = (int32_t)kc.n[1]; w.page = (int32_t)kc.n[2]; w.depth = (int32_t)kc.n[3];
     w.P = (int32_t)table.n[1]; w.max_len = (int32_t)max_len;
-    w.ws_bytes = host.attention_ws(w.B, w.H, w.kv_heads, w.depth, w.max_len);
+    w.ws_bytes = host.attention_ws(w.B, w.H, w.kv_heads, w.depth, w.max_len, w.type);
     Scratch ws;
     if (w.ws_bytes > 0 && !ws.get(w.ws_bytes, stream)) return false;
     w.ws = ws.at;

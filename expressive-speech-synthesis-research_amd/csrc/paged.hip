@@ -1054,12 +1054,16 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const estts_paged_atten
 // parts over all key heads: 61 ragged requests up to 4096 rows of bfloat16 92.8 / 94.7 / 99.7 us, one of 131071 rows 87.0 / 89.4 / 94.4; 128
 // leave half of the CUs idle: 123.8 and 107.0).
 // Requests of up to 1024 rows are not cut: the second launch costs what the shorter sweep gains (4 heads of 64, float32, cut / not cut: one
-// request of 600 rows 7.0 / 6.3 us, of 1000 7.0 / 8.0, of 1500 7.0 / 10.1; and a launch less to issue).  Nor are requests of up to 2048
-// where there is a workgroup for every CU and no second round of many (32 heads on 8 of 128, bfloat16, cut / not cut: 32 requests of
+// request of 600 rows 6.3 / 5.1 us, of 1000 6.4 / 6.7; bfloat16 6.5 / 6.0 and 6.7 / 7.9; and a launch less to issue).  But those of more
+// than 256 KB a key head, where the matrix cores have more to do to a row, are cut while three quarters of the CUs would be idle (32 heads on
+// 8 of 128, bfloat16: one request of 450 rows 8.0 / 7.9, of 600 8.1 / 9.0, of 1000 8.2 / 12.3, four of 1000 9.8 / 13.2, eight 12.4 / 13.0;
+// but sixteen 16.1 / 13.5).  Nor are requests of up to 2048 cut where there is a workgroup for every CU and no second round of many (32 heads on 8 of 128, bfloat16, cut / not cut: 32 requests of
 // 2000 46.9 / 44.1 us, 32 ragged ones 30.4 / 29.4; but 128 168.9 / 164.3 and 128 ragged ones 98.6 / 106.5, 256 185.8 / 188.6).
-int paged_split_target(int B, int H, int kv_heads, int max_len) {
+int paged_split_target(int B, int H, int kv_heads, int depth, int max_len, int type) {
     const long per = (long)kv_heads * ((H / kv_heads + 15) / 16), units = B * per;
-    if (max_len <= 1024 || (units >= 256 && units < 1024 && max_len <= 2048)) return 0;
+    const bool f32 = type == ESTTS_KV_F32, matrix = !f32 || H > FEW_QUERIES * kv_heads;
+    const bool heavy = matrix && units <= 64 && 2LL * max_len * depth * (f32 ? 4 : 2) > 256 * 1024;
+    if ((max_len <= 1024 && !heavy) || (units >= 256 && units < 1024 && max_len <= 2048)) return 0;
     return per < 256 ? (int)(256 / per) : 1;
 }
 
@@ -1159,9 +1163,9 @@ extern "C" int estts_page_write(const estts_page_write_args* args, void* stream)
     return 0;
 }
 
-extern "C" int64_t estts_paged_attention_ws_bytes(int32_t B, int32_t H, int32_t kv_heads, int32_t depth, int32_t max_len) {
+extern "C" int64_t estts_paged_attention_ws_bytes(int32_t B, int32_t H, int32_t kv_heads, int32_t depth, int32_t max_len, int32_t type) {
     if (B <= 0 || H <= 0 || kv_heads <= 0 || H % kv_heads || depth <= 0 || max_len <= 0) return 0;      // (estts_paged_attention says why not)
-    const int target = paged_split_target(B, H, kv_heads, max_len);
+    const int target = paged_split_target(B, H, kv_heads, depth, max_len, type);
     return target ? PagedScratch::bytes(target, H, depth, B) : 0;
 }
 
@@ -1228,7 +1232,7 @@ extern "C" int estts_paged_attention(const estts_paged_attention_args* args, voi
     if (a.max_len == 0 || (int64_t)a.max_len > (int64_t)a.P * a.page) a.max_len = a.P * a.page;
     ESTTS_CHECK_ARG((int64_t)a.B * a.max_len < (1LL << 36) && (int64_t)a.B * a.H < (1LL << 23),
                     "estts_paged_attention: B * max_len must stay below 2^36 and B * H below 2^23");
-    const int target = paged_split_target(a.B, a.H, a.kv_heads, a.max_len);
+    const int target = paged_split_target(a.B, a.H, a.kv_heads, a.depth, a.max_len, a.type);
     const int64_t need = target ? PagedScratch::bytes(target, a.H, a.depth, a.B) : 0;
     ESTTS_CHECK_ARG(need == 0 || (a.ws && a.ws_bytes >= need && !(reinterpret_cast<uintptr_t>(a.ws) & 15)),
                     "estts_paged_attention: this call needs %ld bytes of scratch, 16-byte aligned (given: %ld)", (long)need, (long)a.ws_bytes);

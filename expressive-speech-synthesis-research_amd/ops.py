@@ -807,7 +807,7 @@ def paged_attention(q, k_cache, v_cache, block_table, lengths, ctx, heads, key_m
         sb, ss = key_mask.stride()
     _check_here('paged_attention', 'q k_cache v_cache block_table lengths ctx key_mask', q, k_cache, v_cache, block_table, lengths, ctx, key_mask)
     lib, kind = _lib.load(), KV_TYPES[k_cache.dtype]
-    nbytes = lib.estts_paged_attention_ws_bytes(B, heads, Hk, D, max_len)
+    nbytes = lib.estts_paged_attention_ws_bytes(B, heads, Hk, D, max_len, kind)
     ws = _scratch(nbytes, q.device) if nbytes > 0 else None
     a = _lib.PagedAttentionArgs(q.data_ptr(), ldq, k_cache.data_ptr(), v_cache.data_ptr(), s_page, s_head, s_row,
                                 block_table.data_ptr(), ld, lengths.data_ptr(), _ptr(key_mask), sb, ss, ctx.data_ptr(),

@@ -963,7 +963,7 @@ typedef struct estts_paged_attention_args {
 } estts_paged_attention_args;
 
 int estts_paged_attention(const estts_paged_attention_args* args, void* stream);
-int64_t estts_paged_attention_ws_bytes(int32_t B, int32_t H, int32_t kv_heads, int32_t depth, int32_t max_len);
+int64_t estts_paged_attention_ws_bytes(int32_t B, int32_t H, int32_t kv_heads, int32_t depth, int32_t max_len, int32_t type);
 
 /* ------------------------------------------------------------------------------------------
  * Step programs: a fixed sequence of launches whose arguments depend affinely on a step index (an incremental decoder:

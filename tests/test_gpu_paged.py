@@ -783,7 +783,7 @@ def test_scratch_goes_back_to_the_allocator():
     q, ctx = torch.randn(3, 256, device=DEV), torch.empty(3, 256, device=DEV)
     table, lengths = torch.arange(600, dtype=torch.int32, device=DEV).view(3, 200), dev([3200, 1, 1700])
     slots, free, n_free, new = (torch.empty(6000, dtype=torch.int32, device=DEV), torch.arange(600, dtype=torch.int32, device=DEV), dev([0]), dev([0, 0, 0]))
-    assert ops._lib.load().estts_paged_attention_ws_bytes(3, 4, 2, 64, 3200) > 0 and ops._lib.load().estts_page_plan_ws_bytes(3, 6000) > 0
+    assert ops._lib.load().estts_paged_attention_ws_bytes(3, 4, 2, 64, 3200, 1) > 0 and ops._lib.load().estts_page_plan_ws_bytes(3, 6000) > 0
     torch.cuda.synchronize()
     before = torch.cuda.memory_allocated()
     for stream in (torch.cuda.current_stream(), torch.cuda.Stream()):
