@@ -9,9 +9,9 @@ namespace {
 // ------------------------------------------------------------------------------------------------ page plan
 // Whole-number work on a few kilobytes, bound by latency: a launch, the lengths, the scans, the stack or the table, the maps.  One
 // workgroup scans the requests; the copies and the rows' places are then made by the same workgroup, or by a second launch
-// of as many as it takes where there are more than PLAN_ROWS rows (one workgroup for all: 64 prompts of 2047 rows at most 95 us, now 7.1;
-// 1000 requests that end, grow and arrive, 26000 rows, 84 us, now 10.6).  A step of 32 requests is one launch of 3.2 us, some 2 of which are
-// the launch itself.
+// of as many as it takes where there are more than PLAN_ROWS rows (one workgroup for all / two launches: 64 prompts of 2047 rows at most
+// 67.6 / 6.9 us, 1000 requests that end, grow and arrive, 26000 rows, 67.5 / 10.3).  A step of 32 requests is one launch of 2.8 us, some 2 of
+// which are the launch itself.
 constexpr int PLAN_LDS = 4096;         // requests whose plan fits the LDS (four ints each); beyond that it lives in the caller's scratch
 
 __device__ __forceinline__ int pages_of(int rows, int page) { return (int)(((unsigned)rows + page - 1) / (unsigned)page); }
@@ -121,7 +121,7 @@ __device__ __forceinline__ void carry_out(const estts_page_plan_args& p, const P
         return;
     }
     // Many pages for few threads: a run for each wave, in pieces of one request's pages (at most 64), four in flight; looking each page up
-    // by itself takes a thread 0.8 us a page (100 of 1000 requests of up to 4096 rows end: 17.3 us, like this 13.6).  Only in the kernel of
+    // by itself takes a thread 0.8 us a page (100 of 1000 requests of up to 4096 rows end: 16.3 us, like this 12.5).  Only in the kernel of
     // 1024 threads: the longer code alone costs the others 0.1 to 0.4 us.
     const int lane = first & 63, waves = step >> 6, per = (q.back + 64 * waves - 1) / (64 * waves) * 64;
     int g = __builtin_amdgcn_readfirstlane(first >> 6) * per;
@@ -296,8 +296,8 @@ __global__ __launch_bounds__(256) void page_write_kernel(const estts_page_write_
 // the queries and the weights are split into bfloat16 pieces (three, 24 bits) or float16 pieces (two, 22 bits, behind a power of two that
 // puts the largest element of the query at 2^13 and the largest weight at 2^14), whose products with the pages' values are exact.
 // Scores, maxima, sums and outputs are float32.
-// What bounds it: memory where there are rows enough (5.9 to 6.2 TB/s from 130 MB on; a kernel that only reads gets 6.2), else the chain
-// launch, lengths and table, keys, scores, weights, values, exchange (4.5 us for one request of 100 rows) and some 0.6 to 1.1 us more for
+// What bounds it: memory where there are rows enough (5.9 to 6.4 TB/s from 130 MB on; a kernel that only reads and adds gets 6.2), else the chain
+// launch, lengths and table, keys, scores, weights, values, exchange (3.4 us for one request of 100 rows) and some 0.6 to 1.1 us more for
 // each further tile of a wave.
 
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
@@ -818,8 +818,8 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_attention_kernel(const estts
 // and its 64 float32 matrix instructions a tile (2048 cycles) would set the time of a short request.  On the vector ALU a tile
 // is 64 multiply-adds, 32 data-parallel additions and 8 exponentials a lane and query (some 700 cycles).  Lane (i, g) holds the
 // depth/16 features of rows 4g + j of a half that feature_of says, of K as of V; the sixteen lanes of a row add up its score.
-// One request of 1000 rows, 4 key heads of 64 / 128, matrix cores / here: one query head each 13.4 / 8.0 and 22.2 / 10.7 us, two 13.6 / 10.6
-// and 22.4 / 14.8; 64 such requests, bound by memory: 26.5 / 25.4 and 48.3 / 47.2 us (5.3 and 5.7 TB/s).
+// One request of 1000 rows, 4 key heads of 64 and of 128, matrix cores / here: one query head each 12.8 / 6.7 and 21.2 / 10.4 us, two 12.9 / 8.9
+// and 21.5 / 12.0; 64 such requests, bound by memory: 22.0 / 21.2 and 43.2 / 42.9, two 22.1 / 23.2 and 43.2 / 43.8 us (6.1 TB/s).
 __device__ __forceinline__ float row_sum(float v) {     // over the 16 lanes of a row, to all of them
 #define ESTTS_ROW_STEP(ctrl) v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), ctrl, 0xf, 0xf, false))
     ESTTS_ROW_STEP(0xB1);        // quad_perm [1, 0, 3, 2]
@@ -1051,14 +1051,14 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const estts_paged_atten
 
 // How many parts a call is cut into (0: one workgroup per request and key head, one launch).
 // Parts: one workgroup per CU.  Its four waves keep 64 KB of keys and values in flight, and more parts are more ends to join (256 / 512 / 1024
-// parts over all key heads: 61 ragged requests up to 4096 rows of bfloat16 92.8 / 94.7 / 99.7 us, one of 131071 rows 87.0 / 89.4 / 94.4; 128
-// leave half of the CUs idle: 123.8 and 107.0).
+// parts over all key heads: 61 ragged requests up to 4096 rows of bfloat16 89.3 / 90.0 / 92.4 us, one of 131071 rows 86.2 / 87.5 / 90.5; 128
+// leave half of the CUs idle: 121.1 and 106.1).
 // Requests of up to 1024 rows are not cut: the second launch costs what the shorter sweep gains (4 heads of 64, float32, cut / not cut: one
 // request of 600 rows 6.3 / 5.1 us, of 1000 6.4 / 6.7; bfloat16 6.5 / 6.0 and 6.7 / 7.9; and a launch less to issue).  But those of more
 // than 256 KB a key head, where the matrix cores have more to do to a row, are cut while three quarters of the CUs would be idle (32 heads on
 // 8 of 128, bfloat16: one request of 450 rows 8.0 / 7.9, of 600 8.1 / 9.0, of 1000 8.2 / 12.3, four of 1000 9.8 / 13.2, eight 12.4 / 13.0;
 // but sixteen 16.1 / 13.5).  Nor are requests of up to 2048 cut where there is a workgroup for every CU and no second round of many (32 heads on 8 of 128, bfloat16, cut / not cut: 32 requests of
-// 2000 46.9 / 44.1 us, 32 ragged ones 30.4 / 29.4; but 128 168.9 / 164.3 and 128 ragged ones 98.6 / 106.5, 256 185.8 / 188.6).
+// 2000 45.3 / 43.4 us, 32 ragged ones 28.3 / 28.0; but 128 166.7 / 161.3 and 128 ragged ones 93.7 / 103.0, 256 177.3 / 179.8).
 int paged_split_target(int B, int H, int kv_heads, int depth, int max_len, int type) {
     const long per = (long)kv_heads * ((H / kv_heads + 15) / 16), units = B * per;
     const bool f32 = type == ESTTS_KV_F32, matrix = !f32 || H > FEW_QUERIES * kv_heads;
@@ -1068,9 +1068,10 @@ int paged_split_target(int B, int H, int kv_heads, int depth, int max_len, int t
 }
 
 // Whether the rows are too many for the 256 MB behind the L2s to hold them until the next call, by the most that the lengths can be.
-// Plain / streaming loads of V: 32 heads on 8 of 128, bfloat16, 32 requests of 1000 rows (131 MB) 26.8 / 23.1 us, of 2000 48.2 / 44.3, 61
-// ragged ones up to 4096 (512 MB) 100.4 / 92.9, one of 131071 (537 MB) 97.4 / 87.7 (6.1 TB/s); 8 heads of 64, float32, 200 of 1021 (836 MB)
-// 146.5 / 138.6 (6.0 TB/s).  But 32 ragged ones up to 1000 (65 MB, called again and again) 16.1 / 17.7 and 8 of 1000 (33 MB) 14.3 / 15.9.
+// Plain / streaming loads of V: 32 heads on 8 of 128, bfloat16, 32 requests of 1000 rows (131 MB) 26.3 / 22.4 us, of 2000 48.1 / 43.4, 61
+// ragged ones up to 4096 (512 MB) 98.4 / 89.3, one of 131071 (537 MB) 96.0 / 86.2 (6.2 TB/s); 8 heads of 64, float32, 200 of 1021 (836 MB)
+// 145.9 / 130.9 (6.4 TB/s).  But 32 ragged ones up to 1000 (65 MB, called again and again) 15.4 / 16.4, 8 float32 ones of 1000, 4 heads of 64
+// (16 MB), 8.5 / 10.7.
 bool stream_rows(const estts_paged_attention_args& a) {
     return 2.0 * a.B * a.max_len * a.kv_heads * a.depth * (a.type == ESTTS_KV_F32 ? 4 : 2) > 100e6;
 }
