@@ -151,6 +151,15 @@ struct Scratch {
     }
 };
 
+// Issues a launch without the interpreter's lock: it waits where the stream's queue is full.
+template <typename A>
+bool launch(int (*f)(const A*, void*), const A& args, void* stream) {
+    PyThreadState* state = PyEval_SaveThread();
+    const int rc = f(&args, stream);
+    PyEval_RestoreThread(state);
+    return rc == 0;
+}
+
 bool fits32(int64_t x) { return x >= 0 && x <= INT32_MAX; }
 
 // page_write(k, v, k_cache, v_cache, slots)
@@ -167,7 +176,7 @@ bool page_write(PyObject* const* a, Py_ssize_t n) {
     w.k = k.at; w.v = v.at; w.k_cache = kc.at; w.v_cache = vc.at; w.slots = slots.at;
     w.s_page = kc.s[0]; w.s_head = kc.s[1]; w.s_row = kc.s[2];
     w.T = (int32_t)T; w.n_pages = (int32_t)kc.n[0]; w.heads = (int32_t)kc.n[1]; w.page = (int32_t)kc.n[2]; w.depth = (int32_t)kc.n[3];
-    return host.write(&w, stream) == 0;
+    return launch(host.write, w, stream);
 }
 
 // page_plan(lengths, new, block_table, free_pages, n_free, page, slots, positions, lengths_out, n_free_out, refused)
@@ -199,7 +208,7 @@ bool page_plan(PyObject* const* a, Py_ssize_t n) {
     Scratch ws;
     if (w.ws_bytes > 0 && !ws.get(w.ws_bytes, stream)) return false;
     w.ws = static_cast<int32_t*>(ws.at);
-    return host.plan(&w, stream) == 0;
+    return launch(host.plan, w, stream);
 }
 
 // paged_attention(q, k_cache, v_cache, block_table, lengths, ctx, heads, key_mask, scale, max_len)
@@ -237,7 +246,7 @@ bool paged_attention(PyObject* const* a, Py_ssize_t n) {
     Scratch ws;
     if (w.ws_bytes > 0 && !ws.get(w.ws_bytes, stream)) return false;
     w.ws = ws.at;
-    return host.attention(&w, stream) == 0;
+    return launch(host.attention, w, stream);
 }
 
 // (a tensor that only looks plain, of a function transform, say, throws when its address is asked for)
