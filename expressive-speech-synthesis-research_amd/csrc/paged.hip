@@ -306,7 +306,8 @@ typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
 // request of 600 rows 5.5 / 5.1 us, of 1000 7.1 / 6.7, 64 ragged ones of 600 9.6 / 9.3, one of 100 3.3 / 3.4; on the matrix cores, 32 heads on 8 of
 // 128, bfloat16, one of 1000 12.3 / 12.7, 128 ragged ones of 1000 56.2 / 58.3; cut, 61 ragged ones 89.4 / 90.3).
 constexpr int ATT_WAVES = 4, FEW_WAVES = 8;
-constexpr int FEW_QUERIES = 2;         // query heads per key head up to which float32 pages take the vector ALU
+// query heads per key head up to which the vector ALU takes them (see paged_attention_few_kernel)
+constexpr int few_queries(int esize) { return esize == 4 ? 2 : 1; }
 
 // 16-row halves of a wave's tile
 constexpr int tile_halves(int depth, int esize) { return depth * esize == 512 ? 1 : 2; }
@@ -814,12 +815,14 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_attention_kernel(const estts
     } while (SPLIT && part.left > 0);
 }
 
-// The same for float32 pages and a key head that only one or two query heads read (NQ): most columns of a matrix tile would be empty
-// and its 64 float32 matrix instructions a tile (2048 cycles) would set the time of a short request.  On the vector ALU a tile
+// The same for a key head that only one query head reads, or two of float32 (NQ): most columns of a matrix tile would be empty, and its 64
+// float32 matrix instructions a tile (2048 cycles) or the pieces of 16-bit ones would set the time of a short request.  On the vector ALU a tile
 // is 64 multiply-adds, 32 data-parallel additions and 8 exponentials a lane and query (some 700 cycles).  Lane (i, g) holds the
 // depth/16 features of rows 4g + j of a half that feature_of says, of K as of V; the sixteen lanes of a row add up its score.
 // One request of 1000 rows, 4 key heads of 64 and of 128, matrix cores / here: one query head each 12.8 / 6.7 and 21.2 / 10.4 us, two 12.9 / 8.9
-// and 21.5 / 12.0; 64 such requests, bound by memory: 22.0 / 21.2 and 43.2 / 42.9, two 22.1 / 23.2 and 43.2 / 43.8 us (6.1 TB/s).
+// and 21.5 / 12.0; 64 such requests, bound by memory: 22.0 / 21.2 and 43.2 / 42.9, two 22.1 / 23.2 and 43.2 / 43.8 us (6.1 TB/s).  bfloat16, 4 key
+// heads of 32 / 64 / 128, one query head each: one request of 400 rows 4.8 / 4.2, 5.4 / 5.1 and 7.3 / 6.2 us, 128 of 1000 12.8 / 13.7, 21.9 / 23.4 and
+// 43.9 / 43.8; two query heads each: 4.8 / 5.3, 5.4 / 6.6 and 7.4 / 8.4, 12.8 / 16.0, 22.2 / 24.1 and 44.3 / 46.9, so the matrix cores keep those.
 __device__ __forceinline__ float row_sum(float v) {     // over the 16 lanes of a row, to all of them
 #define ESTTS_ROW_STEP(ctrl) v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), ctrl, 0xf, 0xf, false))
     ESTTS_ROW_STEP(0xB1);        // quad_perm [1, 0, 3, 2]
@@ -830,11 +833,12 @@ __device__ __forceinline__ float row_sum(float v) {     // over the 16 lanes of 
     return v;
 }
 
-template <int DH, bool MASK, bool STREAM, bool SPLIT, int NQ, int NW>
+template <typename T, int DH, bool MASK, bool STREAM, bool SPLIT, int NQ, int NW>
 __global__ __launch_bounds__(NW * 64, 2) void paged_attention_few_kernel(const estts_paged_attention_args p, const int target) {
-    constexpr uint32_t ALL_ROWS = tile_halves(DH, 4) == 2 ? 0xFFFFFFFFu : 0xFFFFu;
-    constexpr int HALVES = tile_halves(DH, 4), TILE = 16 * HALVES, NV = DH / 16, RUN = NV < 4 ? NV : 4;
-    typedef __attribute__((ext_vector_type(RUN))) float run_t;
+    constexpr int ES = (int)sizeof(T), HALVES = tile_halves(DH, ES), TILE = 16 * HALVES;
+    constexpr uint32_t ALL_ROWS = HALVES == 2 ? 0xFFFFFFFFu : 0xFFFFu;
+    constexpr int NV = DH / 16, RUN = NV * ES < 16 ? NV : 16 / ES, RUNS = NV / RUN;        // features of a row per lane, of one load
+    typedef __attribute__((ext_vector_type(RUN))) T run_t;
     __shared__ __attribute__((aligned(16))) float o_s[NW][NQ][DH];
     __shared__ float m_s[NW][NQ], l_s[NW][NQ];
     const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
@@ -846,35 +850,32 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_attention_few_kernel(const e
     do {
         const PagedSegment seg = part.next(p, u.h0 == 0 && threadIdx.x == 0 ? ws.items : nullptr);
         const int b = seg.b, begin = seg.begin, end = seg.end;
-        PageWalk<HALVES, NW> walk(p, b, begin, wave, 4);
+        PageWalk<HALVES, NW> walk(p, b, begin, wave, ES);
         const float qs = p.scale * 1.4426950408889634f;
         float qx[NQ][NV];
 #pragma unroll
         for (int n = 0; n < NQ; ++n)
 #pragma unroll
-            for (int e = 0; e < NV; ++e) qx[n][e] = p.q[b * p.ldq + (long)(u.h0 + min(n, u.heads - 1)) * DH + feature_of<DH, 4>(i, e)] * qs;
+            for (int e = 0; e < NV; ++e) qx[n][e] = p.q[b * p.ldq + (long)(u.h0 + min(n, u.heads - 1)) * DH + feature_of<DH, ES>(i, e)] * qs;
         const int n_tiles = (end - begin + TILE - 1) / TILE;
         const int n_mine = __builtin_amdgcn_readfirstlane(n_tiles > wave ? (n_tiles - wave + NW - 1) / NW : 0);
-        const char* kbase = static_cast<const char*>(p.k_cache) + u.hk * p.s_head * 4;
-        const char* vbase = static_cast<const char*>(p.v_cache) + u.hk * p.s_head * 4;
-        const int row_bytes = (int)(p.s_row * 4);
-        int lane_at = 4 * g * row_bytes + i * 4 * RUN;      // (0 behind the last tile: one line for the whole wave)
+        const char* kbase = static_cast<const char*>(p.k_cache) + u.hk * p.s_head * ES;
+        const char* vbase = static_cast<const char*>(p.v_cache) + u.hk * p.s_head * ES;
+        const int row_bytes = (int)(p.s_row * ES);
+        int lane_at = 4 * g * row_bytes + i * ES * RUN;      // (0 behind the last tile: one line for the whole wave)
 
-        float kr[HALVES][4][NV], vr[HALVES][4][NV];
+        run_t kr[HALVES][4][RUNS], vr[HALVES][4][RUNS];
         [[maybe_unused]] float mk;
-        auto load = [&](const char* base, float (&r)[HALVES][4][NV], auto hint) {
+        auto load = [&](const char* base, run_t (&r)[HALVES][4][RUNS], auto hint) {
 #pragma unroll
             for (int s = 0; s < HALVES; ++s)
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
 #pragma unroll
-                    for (int x = 0; x < NV; x += RUN) {
-                        const run_t* at = reinterpret_cast<const run_t*>(base + walk.at[s] + (unsigned)(lane_at + 64 * x + j * row_bytes));
-                        run_t t;
-                        if constexpr (decltype(hint)::value) t = __builtin_nontemporal_load(at);
-                        else t = *at;
-#pragma unroll
-                        for (int e = 0; e < RUN; ++e) r[s][j][x + e] = t[e];
+                    for (int x = 0; x < RUNS; ++x) {
+                        const run_t* at = reinterpret_cast<const run_t*>(base + walk.at[s] + (unsigned)(lane_at + 16 * ES * RUN * x + j * row_bytes));
+                        if constexpr (decltype(hint)::value) r[s][j][x] = __builtin_nontemporal_load(at);
+                        else r[s][j][x] = *at;
                     }
         };
         auto load_k = [&]() { load(kbase, kr, std::false_type()); };
@@ -910,9 +911,9 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_attention_few_kernel(const e
                     for (int s = 0; s < HALVES; ++s)
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
-                            float t = kr[s][j][0] * qx[n][0];
+                            float t = (float)kr[s][j][0][0] * qx[n][0];
 #pragma unroll
-                            for (int e = 1; e < NV; ++e) t = fmaf(kr[s][j][e], qx[n][e], t);
+                            for (int e = 1; e < NV; ++e) t = fmaf((float)kr[s][j][e / RUN][e % RUN], qx[n][e], t);
                             sc[n][s][j] = row_sum(t);
                         }
                 uint32_t rows_in = 0;
@@ -936,7 +937,8 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_attention_few_kernel(const e
 #pragma unroll
                             for (int n = 0; n < NQ; ++n) sc[n][s][j] = in ? sc[n][s][j] : -INFINITY;
 #pragma unroll
-                            for (int e = 0; e < NV; ++e) vr[s][j][e] = in ? vr[s][j][e] : 0.0f;
+                            for (int x = 0; x < RUNS; ++x)
+                                if (!in) vr[s][j][x] = (run_t)(T)0.0f;
                         }
                 }
 #pragma unroll
@@ -962,7 +964,7 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_attention_few_kernel(const e
                             const float w = __builtin_amdgcn_exp2f(sc[n][s][j] - base);
                             l[n] += w;
 #pragma unroll
-                            for (int e = 0; e < NV; ++e) o[n][e] = fmaf(w, vr[s][j][e], o[n][e]);
+                            for (int e = 0; e < NV; ++e) o[n][e] = fmaf(w, (float)vr[s][j][e / RUN][e % RUN], o[n][e]);
                         }
                 }
                 load_v();
@@ -977,7 +979,7 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_attention_few_kernel(const e
             for (int e = 0; e < NV; ++e) {
                 o[n][e] += lane_xor16(o[n][e]);
                 o[n][e] += lane_xor32(o[n][e]);
-                if (g == 0) o_s[wave][n][feature_of<DH, 4>(i, e)] = o[n][e];
+                if (g == 0) o_s[wave][n][feature_of<DH, ES>(i, e)] = o[n][e];
             }
         }
         __syncthreads();
@@ -1054,15 +1056,17 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const estts_paged_atten
 // parts over all key heads: 61 ragged requests up to 4096 rows of bfloat16 89.3 / 90.0 / 92.4 us, one of 131071 rows 86.2 / 87.5 / 90.5; 128
 // leave half of the CUs idle: 121.1 and 106.1).
 // Requests of up to 1024 rows are not cut: the second launch costs what the shorter sweep gains (4 heads of 64, float32, cut / not cut: one
-// request of 600 rows 6.3 / 5.1 us, of 1000 6.4 / 6.7; bfloat16 6.5 / 6.0 and 6.7 / 7.9; and a launch less to issue).  But those of more
-// than 256 KB a key head, where the matrix cores have more to do to a row, are cut while three quarters of the CUs would be idle (32 heads on
-// 8 of 128, bfloat16: one request of 450 rows 8.0 / 7.9, of 600 8.1 / 9.0, of 1000 8.2 / 12.3, four of 1000 9.8 / 13.2, eight 12.4 / 13.0;
-// but sixteen 16.1 / 13.5).  Nor are requests of up to 2048 cut where there is a workgroup for every CU and no second round of many (32 heads on 8 of 128, bfloat16, cut / not cut: 32 requests of
-// 2000 45.3 / 43.4 us, 32 ragged ones 28.3 / 28.0; but 128 166.7 / 161.3 and 128 ragged ones 93.7 / 103.0, 256 177.3 / 179.8).
+// request of 600 rows 6.2 / 5.1 us, of 1000 6.4 / 6.7; and a launch less to issue).  But few wide ones are, from 512 KB a key head on, or
+// 256 KB where the matrix cores have more to do to a row (4 heads of 128, float32: one request of 500 rows 6.6 / 6.7 us, of 1000 6.5 / 10.4, eight
+// ragged ones 9.8 / 12.9, sixteen 12.9 / 13.5 and of 600 11.0 / 9.7; 32 heads on 8 of 128, bfloat16: one of 450 rows 8.0 / 7.9, of 1000 8.2 / 12.3,
+// eight 12.4 / 13.0, sixteen 16.1 / 13.5).  Nor are requests of up to 2048 cut where there is a workgroup for every CU and no second round of
+// many (32 heads on 8 of 128, bfloat16, cut / not cut: 32 requests of 2000 45.3 / 43.4 us, 32 ragged ones 28.3 / 28.0; but 128 166.7 / 161.3
+// and 128 ragged ones 93.7 / 103.0, 256 177.3 / 179.8).
 int paged_split_target(int B, int H, int kv_heads, int depth, int max_len, int type) {
     const long per = (long)kv_heads * ((H / kv_heads + 15) / 16), units = B * per;
-    const bool f32 = type == ESTTS_KV_F32, matrix = !f32 || H > FEW_QUERIES * kv_heads;
-    const bool heavy = matrix && units <= 64 && 2LL * max_len * depth * (f32 ? 4 : 2) > 256 * 1024;
+    const int esize = type == ESTTS_KV_F32 ? 4 : 2;
+    const bool matrix = H > few_queries(esize) * kv_heads;
+    const bool heavy = units <= (matrix ? 64 : 32) && 2LL * max_len * depth * esize > (matrix ? 256 : 512) * 1024;
     if ((max_len <= 1024 && !heavy) || (units >= 256 && units < 1024 && max_len <= 2048)) return 0;
     return per < 256 ? (int)(256 / per) : 1;
 }
@@ -1175,18 +1179,11 @@ static void launch_paged_attention(const estts_paged_attention_args& a, int targ
     const int group = a.H / a.kv_heads, n_group = (group + 15) / 16;
     const int units = (target ? target : a.B) * a.kv_heads;
     const dim3 grid(n_group > 1 ? (units + 7) / 8 * 8 * n_group : units), block(ATT_WAVES * 64);
-    if constexpr (sizeof(T) == 4) {
-        constexpr int NW = SPLIT ? ATT_WAVES : FEW_WAVES;
-        if (group == 1) {
-            ESTTS_LAUNCH((paged_attention_few_kernel<DH, MASK, STREAM, SPLIT, 1, NW>), grid, dim3(NW * 64), 0, stream, a, target);
-            return;
-        }
-        if (group <= FEW_QUERIES) {
-            ESTTS_LAUNCH((paged_attention_few_kernel<DH, MASK, STREAM, SPLIT, FEW_QUERIES, NW>), grid, dim3(NW * 64), 0, stream, a, target);
-            return;
-        }
-    }
-    ESTTS_LAUNCH((paged_attention_kernel<T, DH, MASK, STREAM, SPLIT, ATT_WAVES>), grid, block, 0, stream, a, target);
+    constexpr int NW = SPLIT ? ATT_WAVES : FEW_WAVES;
+    constexpr int FEW = few_queries((int)sizeof(T));
+    if (group == 1) ESTTS_LAUNCH((paged_attention_few_kernel<T, DH, MASK, STREAM, SPLIT, 1, NW>), grid, dim3(NW * 64), 0, stream, a, target);
+    else if (group <= FEW) ESTTS_LAUNCH((paged_attention_few_kernel<T, DH, MASK, STREAM, SPLIT, FEW, NW>), grid, dim3(NW * 64), 0, stream, a, target);
+    else ESTTS_LAUNCH((paged_attention_kernel<T, DH, MASK, STREAM, SPLIT, ATT_WAVES>), grid, block, 0, stream, a, target);
 }
 
 template <typename T, int DH, bool SPLIT>
