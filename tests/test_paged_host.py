@@ -270,3 +270,15 @@ def test_lane_loads_cover_each_row_once(depth, esize):
     last_v = 4 * 3 * row_bytes + 15 * run * esize + 256 * ((nv - 1) // run) + 3 * row_bytes + run * esize
     last_k = 15 * row_bytes + 16 * 3 + 64 * (depth * esize // 64 - 1) + 16
     assert last_v == last_k == half_bytes
+
+
+@pytest.mark.parametrize('B,heads,kv_heads,depth,max_len,type,cut', [
+    (1, 4, 4, 64, 1024, 0, False), (1, 4, 4, 64, 1025, 0, True), (1, 4, 4, 128, 512, 0, False), (1, 4, 4, 128, 513, 0, True), (8, 4, 4, 128, 600, 0, True),
+    (9, 4, 4, 128, 600, 0, False), (1, 12, 4, 128, 256, 0, False), (1, 12, 4, 128, 257, 0, True), (1, 32, 8, 128, 513, 1, True), (8, 32, 8, 128, 513, 2, True),
+    (9, 32, 8, 128, 513, 1, False), (1, 8, 8, 128, 1000, 1, False), (1, 64, 1, 64, 1000, 2, False), (32, 8, 8, 64, 2048, 0, False), (32, 8, 8, 64, 2049, 0, True),
+    (31, 8, 8, 64, 2048, 0, True), (128, 8, 8, 64, 2048, 0, True), (1, 600, 600, 32, 5000, 1, True)])
+def test_which_calls_are_cut(B, heads, kv_heads, depth, max_len, type, cut):
+    lib = _lib.load()
+    nbytes = lib.estts_paged_attention_ws_bytes(B, heads, kv_heads, depth, max_len, type)
+    parts = max(1, 256 // (kv_heads * -(-heads // kv_heads // 16)))
+    assert nbytes == (2 * parts * heads * (depth + 2) * 4 + 8 * B if cut else 0)
