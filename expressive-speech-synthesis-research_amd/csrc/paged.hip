@@ -6,15 +6,34 @@
 
 namespace {
 
+// x / d for x < 2^bits without a division, whose thirty instructions stand in the way of the first loads of a short call (one request of
+// 100 rows 3.35 / 3.17 us, three of up to 2500, cut, 6.45 / 6.16): with s = ceil(log2 d) and
+// m = ceil(2^(bits + s) / d), m d = 2^(bits + s) + e, e < d <= 2^s, so x m / 2^(bits + s) is less than 1/d above x / d.  bits + s <= 62.
+struct Divisor {
+    uint32_t m; int shift;
+    __device__ __forceinline__ int of(uint32_t x) const { return (int)(((uint64_t)x * m) >> shift); }
+};
+Divisor divisor(uint32_t d, int bits) {
+    int s = 0;
+    while ((1ULL << s) < d) ++s;
+    return {(uint32_t)(((1ULL << (bits + s)) + d - 1) / d), bits + s};
+}
+
+// x / page for any x below 2^32: pages are multiples of 16 rows
+struct PageSize {
+    Divisor sixteenths; int page;
+    __device__ __forceinline__ int of(uint32_t x) const { return sixteenths.of(x >> 4); }
+    __device__ __forceinline__ int holding(int rows) const { return of((uint32_t)rows + page - 1); }        // pages that so many rows take
+};
+PageSize page_size(int page) { return {divisor((uint32_t)page / 16, 28), page}; }
+
 // ------------------------------------------------------------------------------------------------ page plan
 // Whole-number work on a few kilobytes, bound by latency: a launch, the lengths, the scans, the stack or the table, the maps.  One
 // workgroup scans the requests; the copies and the rows' places are then made by the same workgroup, or by a second launch
 // of as many as it takes where there are more than PLAN_ROWS rows (one workgroup for all / two launches: 64 prompts of 2047 rows at most
-// 67.6 / 6.9 us, 1000 requests that end, grow and arrive, 26000 rows, 67.5 / 10.3).  A step of 32 requests is one launch of 2.8 us, some 2 of
+// 67.6 / 6.7 us, 1000 requests that end, grow and arrive, 26000 rows, 67.5 / 9.9).  A step of 32 requests is one launch of 2.8 us, some 2 of
 // which are the launch itself.
 constexpr int PLAN_LDS = 4096;         // requests whose plan fits the LDS (four ints each); beyond that it lives in the caller's scratch
-
-__device__ __forceinline__ int pages_of(int rows, int page) { return (int)(((unsigned)rows + page - 1) / (unsigned)page); }
 
 // A value from another lane, 0 where there is none: CTRL says which (row_shr 1, 2, 4, 8: that many lanes below in the row of 16; row_bcast 15, 31:
 // the last lane of the row, of the half wave before), ROWS which rows of 16 take it.
@@ -77,13 +96,14 @@ struct PagePlan {
     const int* len_of;         // its length, complemented where it gets no rows
     int height0, back, taken;  // the stack before the call, pages that come back to it, pages that are then taken off it
 };
+struct PageDivisors { PageSize page; Divisor row; };           // (row: of a padded map)
 constexpr int PLAN_HEAD = 4;   // scratch of a plan in two launches: height0, back, taken, then the four arrays
 
 // The copies that a plan asks for, in any order and by any thread: every source is as the call found it.  Place e of the stack with the
 // given-back pages on it is free_pages[e] below height0, above it the page of an ended request; a row's page is in the table if the
 // request held it already, else on the stack.
 template <bool PADDED, bool RUNS>
-__device__ __forceinline__ void carry_out(const estts_page_plan_args& p, const PagePlan& q, const int first, const int step) {
+__device__ __forceinline__ void carry_out(const estts_page_plan_args& p, const PageDivisors& by, const PagePlan& q, const int first, const int step) {
     auto given_back = [&](int g) {
         const int b = first_past(q.back_end, p.B, g);
         return p.block_table[b * p.ld_table + (g - (b ? q.back_end[b - 1] : 0))];
@@ -96,16 +116,16 @@ __device__ __forceinline__ void carry_out(const estts_page_plan_args& p, const P
         if (x >= rows) {
             const int g = x - rows, b = first_past(q.page_end, p.B, g);
             const int i = g - (b ? q.page_end[b - 1] : 0);
-            p.block_table[b * p.ld_table + pages_of(q.len_of[b], p.page) + i] = on_stack(height - 1 - g);
+            p.block_table[b * p.ld_table + by.page.holding(q.len_of[b]) + i] = on_stack(height - 1 - g);
         } else if (x < p.T) {
-            const int b = PADDED ? (int)((unsigned)x / (unsigned)p.R) : first_past(q.row_end, p.B, x);
+            const int b = PADDED ? by.row.of(x) : first_past(q.row_end, p.B, x);
             int slot = -1, pos = -1;
             const int len = b < p.B ? q.len_of[b] : -1;
             if (len >= 0) {
                 const int i = PADDED ? x - b * p.R : x - (b ? q.row_end[b - 1] : 0);
                 if (!PADDED || i < q.row_end[b]) {
                     pos = len + i;
-                    const int j = (int)((unsigned)pos / (unsigned)p.page), fresh = j - pages_of(len, p.page);
+                    const int j = by.page.of(pos), fresh = j - by.page.holding(len);
                     const int id = fresh < 0 ? p.block_table[b * p.ld_table + j] : on_stack(height - 1 - ((b ? q.page_end[b - 1] : 0) + fresh));
                     if (id >= 0 && id < p.n_pages) slot = id * p.page + (pos - j * p.page);
                 }
@@ -155,7 +175,7 @@ __device__ __forceinline__ void carry_out(const estts_page_plan_args& p, const P
 
 // The scans, by one workgroup; then the copies, unless they are left to page_copy_kernel (SPLIT; the plan goes to p.ws).
 template <int NT, bool LDS, bool PADDED, bool SPLIT>
-__global__ __launch_bounds__(NT) void page_plan_kernel(const estts_page_plan_args p) {
+__global__ __launch_bounds__(NT) void page_plan_kernel(const estts_page_plan_args p, const PageDivisors by) {
     __shared__ int back_s[NT / 64], need_s[2][NT / 64];
     __shared__ long long rows_s[NT / 64];
     __shared__ int taken_s, refused_s;
@@ -177,7 +197,7 @@ __global__ __launch_bounds__(NT) void page_plan_kernel(const estts_page_plan_arg
         const int n = b < p.B ? p.n_new[b] : 0;
         const int len = b < p.B ? min(max(p.lengths[b], 0), cap) : 0;
         int back_total;
-        const int upto = back + block_scan<NT>(n < 0 ? pages_of(len, p.page) : 0, back_s, back_total);
+        const int upto = back + block_scan<NT>(n < 0 ? by.page.holding(len) : 0, back_s, back_total);
         long long rows_total = 0, rows_upto = 0;
         if constexpr (PADDED) { if (b0 + NT < p.B) __syncthreads(); }       // (for back_s)
         else rows_upto = rows_before + block_scan<NT>((long long)max(n, 0), rows_s, rows_total);
@@ -199,7 +219,7 @@ __global__ __launch_bounds__(NT) void page_plan_kernel(const estts_page_plan_arg
         const int n = b < p.B ? p.n_new[b] : 0;
         const int mark = b < p.B ? mark_of[b] : 0, len = mark < 0 ? ~mark : mark;
         const bool fits = b < p.B && n >= 0 && mark >= 0 && len + (long long)n <= cap;
-        const int need = fits ? pages_of(len + n, p.page) - pages_of(len, p.page) : 0;
+        const int need = fits ? by.page.holding(len + n) - by.page.holding(len) : 0;
         int need_total;
         const int upto = asked + block_scan<NT>(need, need_s[turn], need_total);
         const bool granted = fits && (need == 0 || upto <= height);
@@ -221,12 +241,12 @@ __global__ __launch_bounds__(NT) void page_plan_kernel(const estts_page_plan_arg
     if constexpr (SPLIT) {
         if (tid == 0) { p.ws[0] = height0; p.ws[1] = back; p.ws[2] = taken; }
     } else {
-        carry_out<PADDED, NT == 1024>(p, {row_end, back_end, page_end, len_of, height0, back, taken}, tid, NT);
+        carry_out<PADDED, NT == 1024>(p, by, {row_end, back_end, page_end, len_of, height0, back, taken}, tid, NT);
     }
 }
 
 template <bool LDS, bool PADDED>
-__global__ __launch_bounds__(256) void page_copy_kernel(const estts_page_plan_args p) {
+__global__ __launch_bounds__(256) void page_copy_kernel(const estts_page_plan_args p, const PageDivisors by) {
     __shared__ __attribute__((aligned(16))) int plan_s[LDS ? 4 * PLAN_LDS : 4];
     const int* plan = p.ws + PLAN_HEAD;
     const int height0 = p.ws[0], back = p.ws[1], taken = p.ws[2];
@@ -237,7 +257,7 @@ __global__ __launch_bounds__(256) void page_copy_kernel(const estts_page_plan_ar
         __syncthreads();
         plan = plan_s;
     }
-    carry_out<PADDED, false>(p, {plan, plan + p.B, plan + 2 * (long)p.B, plan + 3 * (long)p.B, height0, back, taken}, blockIdx.x * 256 + threadIdx.x, gridDim.x * 256);
+    carry_out<PADDED, false>(p, by, {plan, plan + p.B, plan + 2 * (long)p.B, plan + 3 * (long)p.B, height0, back, taken}, blockIdx.x * 256 + threadIdx.x, gridDim.x * 256);
 }
 
 // ------------------------------------------------------------------------------------------------ rows into the pages
@@ -297,7 +317,7 @@ __global__ __launch_bounds__(256) void page_write_kernel(const estts_page_write_
 // puts the largest element of the query at 2^13 and the largest weight at 2^14), whose products with the pages' values are exact.
 // Scores, maxima, sums and outputs are float32.
 // What bounds it: memory where there are rows enough (5.9 to 6.4 TB/s from 130 MB on; a kernel that only reads and adds gets 6.2), else the chain
-// launch, lengths and table, keys, scores, weights, values, exchange (3.4 us for one request of 100 rows) and some 0.6 to 1.1 us more for
+// launch, lengths and table, keys, scores, weights, values, exchange (3.2 us for one request of 100 rows) and some 0.6 to 1.1 us more for
 // each further tile of a wave.
 
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
@@ -368,47 +388,53 @@ __device__ __forceinline__ int request_rows(const estts_paged_attention_args& p,
 // in units of UNIT, are one line that is cut into equal parts, so that long and short requests keep the chip equally busy and no part
 // is last; the host knows no lengths, the parts follow from them on the GPU.  A part holds whole requests, the end of one that began in
 // an earlier part and the beginning of one that goes on in a later part: two places of scratch a part, 2k and 2k + 1, hold the latter two.
+// What the host works out of a call's arguments: the page size, query heads per key head, groups of them, and how to divide by kv_heads and target.
+struct PagedCall { PageSize page; int group, n_group, target; Divisor kv_heads, by_target; };
 struct PagedSegment { int b, begin, end, place; bool whole; };      // rows [begin, end) of request b; place: of the scratch, unless whole
 
 template <int NT, int UNIT, bool SPLIT>
 struct PagedPart {
-    int k, parts, b, off, left, total, at;      // requests from b on, of b the units from off on, left units in all; at: place of unit off of b in the line
+    int k, b, off, left, at;                    // requests from b on, of b the units from off on, left units in all; at: place of unit off of b in the line
+    int parts, total;                           // part k holds units [floor(k total / parts), floor((k + 1) total / parts)) of the line
 
     static __device__ __forceinline__ int units_of(int rows) { return max((rows + UNIT - 1) / UNIT, 1); }      // (a request without rows still gets its zeros)
 
-    __device__ __forceinline__ bool find(const estts_paged_attention_args& p, int part, int target) {
-        int first = part, from = 0, to = 0, skip = 0, all = 1, n_parts = 1;
+    // that unit x of the line is in: floor(((x + 1) parts - 1) / total), in float64 (below 2^38 over below 2^30: a quotient that is no whole number
+    // is 2^-30 away from the next)
+    __device__ __forceinline__ int part_of(int x) const { return (int)(((x + 1.0) * parts - 1.0) / total); }
+
+    __device__ __forceinline__ bool find(const estts_paged_attention_args& p, const PagedCall& c, int part) {
+        int first = part, skip = 0;
+        at = left = total = 0;
+        parts = p.B;
         if constexpr (SPLIT) {
             __shared__ int scan_s[NT / 64], found_s[2];
             const int per = (p.B + NT - 1) / NT, b0 = threadIdx.x * per, b1 = min(b0 + per, p.B);
             int mine = 0;                       // (the sum over all is at most 2^30: the caller keeps B * max_len below 2^36)
             for (int x = b0; x < b1; ++x) mine += units_of(request_rows(p, x));
-            const int upto = block_scan<NT>(mine, scan_s, all);
-            n_parts = min(target, all);
-            from = (int)((long)part * all / n_parts);
-            to = (int)((long)(part + 1) * all / n_parts);
-            if (part < n_parts && upto > from && upto - mine <= from) {
+            const int upto = block_scan<NT>(mine, scan_s, total);
+            parts = min(c.target, total);
+            const int share = total < c.target ? 1 : c.by_target.of(total), extra = total - share * parts;     // (extra < target <= 256)
+            at = part * share + c.by_target.of(part * extra);
+            left = share + c.by_target.of((part + 1) * extra) - c.by_target.of(part * extra);
+            if (part < parts && upto > at && upto - mine <= at) {
                 int x = b0, before = upto - mine;
                 for (; x < b1 - 1; ++x) {
                     const int n = units_of(request_rows(p, x));
-                    if (before + n > from) break;
+                    if (before + n > at) break;
                     before += n;
                 }
                 found_s[0] = x;
-                found_s[1] = from - before;
+                found_s[1] = at - before;
             }
             __syncthreads();
             first = found_s[0];
             skip = found_s[1];
         }
         k = part;
-        parts = n_parts;
-        total = all;
         b = __builtin_amdgcn_readfirstlane(first);
         off = __builtin_amdgcn_readfirstlane(skip);
-        left = to - from;
-        at = from;
-        return part < (SPLIT ? n_parts : p.B);
+        return part < parts;
     }
 
     // the next rows to do; items (of the first key head's workgroups): where the join finds request b
@@ -416,8 +442,7 @@ struct PagedPart {
         const int rows = __builtin_amdgcn_readfirstlane(request_rows(p, b));
         const int n = units_of(rows), take = SPLIT ? min(n - off, left) : n;
         const PagedSegment s = {b, off * UNIT, min(rows, (off + take) * UNIT), 2 * k + (off == 0), !SPLIT || take == n};
-        // unit x of the line is in part floor(((x + 1) parts - 1) / total)
-        if (SPLIT && off == 0 && items) items[b] = make_int2(k, take == n ? 1 : (int)((((long)at + n) * parts - 1) / total) - k + 1);
+        if (SPLIT && off == 0 && items) items[b] = make_int2(k, take == n ? 1 : part_of(at + n - 1) - k + 1);
         left -= take;
         at += take;
         off = 0;
@@ -446,13 +471,14 @@ struct PageWalk {
     static constexpr int TILE = 16 * HALVES, PER_BLOCK = 64 / HALVES;
     const int* table;
     long s_page, s_row;                                 // in bytes
-    int page, n_pages, max_len, begin, wave, lane;
+    PageSize page;
+    int n_pages, max_len, begin, wave, lane;
     int entry, next_entry, at_lo, at_hi;                // of this lane's half: its page, its byte offset (negative: no such page)
     long at[HALVES];                                    // of the tile last located
     bool ok[HALVES];
 
-    __device__ __forceinline__ PageWalk(const estts_paged_attention_args& p, int b, int begin_, int wave_, int esize)
-        : table(p.block_table + b * p.ld_table), s_page(p.s_page * esize), s_row(p.s_row * esize), page(p.page), n_pages(p.n_pages),
+    __device__ __forceinline__ PageWalk(const estts_paged_attention_args& p, const PagedCall& c, int b, int begin_, int wave_, int esize)
+        : table(p.block_table + b * p.ld_table), s_page(p.s_page * esize), s_row(p.s_row * esize), page(c.page), n_pages(p.n_pages),
           max_len(p.max_len), begin(begin_), wave(wave_), lane(threadIdx.x & 63) {
         entry = entry_of(0);
         next_entry = entry_of(1);
@@ -463,11 +489,11 @@ struct PageWalk {
         return begin + ((block * PER_BLOCK + lane / HALVES) * NW + wave) * TILE + 16 * (lane % HALVES);
     }
     // (bounded by max_len, which the host knows, not by the length: the table and the lengths are read side by side)
-    __device__ __forceinline__ int entry_of(int block) const { return table[min(half_row(block), max_len - 1) / page]; }
+    __device__ __forceinline__ int entry_of(int block) const { return table[page.of(min(half_row(block), max_len - 1))]; }
     __device__ __forceinline__ void place(int block) {
         const int r = half_row(block);
         const bool there = entry >= 0 && entry < n_pages && r < max_len;
-        const long x = there ? entry * s_page + (long)(r % page) * s_row : -1L;
+        const long x = there ? entry * s_page + (long)(r - page.of(r) * page.page) * s_row : -1L;
         at_lo = (int)(x & 0xFFFFFFFFL);
         at_hi = (int)(x >> 32);
     }
@@ -492,19 +518,18 @@ struct PageWalk {
 template <int MAXQ>
 struct PagedUnit {
     int part, hk, h0, heads;
-    __device__ __forceinline__ PagedUnit(const estts_paged_attention_args& p) {
+    __device__ __forceinline__ PagedUnit(const estts_paged_attention_args& p, const PagedCall& c) {
         // query groups of one key head next to each other on one XCD (workgroups whose numbers agree mod 8), whose L2 then holds the rows
-        const int group = p.H / p.kv_heads, n_group = (group + MAXQ - 1) / MAXQ;
         int unit = blockIdx.x, q = 0;
-        if (n_group > 1) {
+        if (MAXQ > 2 && c.n_group > 1) {
             const int k = unit >> 3;
-            q = k % n_group;
-            unit = (k / n_group) * 8 + (unit & 7);
+            q = k % c.n_group;
+            unit = (k / c.n_group) * 8 + (unit & 7);
         }
-        part = unit / p.kv_heads;
+        part = c.kv_heads.of(unit);
         hk = unit - part * p.kv_heads;
-        heads = min(MAXQ, group - q * MAXQ);
-        h0 = hk * group + q * MAXQ;
+        heads = min(MAXQ, c.group - q * MAXQ);
+        h0 = hk * c.group + q * MAXQ;
     }
 };
 
@@ -545,10 +570,10 @@ __device__ __forceinline__ void join_waves(const estts_paged_attention_args& p, 
     }
 }
 
-// SPLIT: the rows are cut into `target` parts.  (A kernel for each: the code of the cutting alone, not run, cost a short request 0.4 to 0.7 us,
+// SPLIT: the rows are cut into c.target parts.  (A kernel for each: the code of the cutting alone, not run, cost a short request 0.4 to 0.7 us,
 // one of 100 rows float32 4.2 / 3.6.)
 template <typename T, int DH, bool MASK, bool STREAM, bool SPLIT, int NW>
-__global__ __launch_bounds__(NW * 64, 2) void paged_attention_kernel(const estts_paged_attention_args p, const int target) {
+__global__ __launch_bounds__(NW * 64, 2) void paged_attention_kernel(const estts_paged_attention_args p, const PagedCall c) {
     constexpr bool F32 = sizeof(T) == 4;
     constexpr int HALVES = tile_halves(DH, sizeof(T));
     constexpr int TILE = 16 * HALVES;
@@ -560,15 +585,15 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_attention_kernel(const estts
 
     const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const PagedUnit<16> u(p);
+    const PagedUnit<16> u(p, c);
     const int heads = u.heads, h0 = u.h0;
-    const PagedScratch ws(p.ws, target, p.H, DH);
+    const PagedScratch ws(p.ws, c.target, p.H, DH);
     PagedPart<NW * 64, TILE * NW, SPLIT> part;
-    if (!part.find(p, u.part, target)) return;
+    if (!part.find(p, c, u.part)) return;
     do {
         const PagedSegment seg = part.next(p, h0 == 0 && threadIdx.x == 0 ? ws.items : nullptr);
         const int b = seg.b, begin = seg.begin, end = seg.end;
-        PageWalk<HALVES, NW> walk(p, b, begin, wave, sizeof(T));
+        PageWalk<HALVES, NW> walk(p, c, b, begin, wave, sizeof(T));
 
         // ---- queries
         const float qs = p.scale * 1.4426950408889634f;
@@ -834,7 +859,7 @@ __device__ __forceinline__ float row_sum(float v) {     // over the 16 lanes of 
 }
 
 template <typename T, int DH, bool MASK, bool STREAM, bool SPLIT, int NQ, int NW>
-__global__ __launch_bounds__(NW * 64, 2) void paged_attention_few_kernel(const estts_paged_attention_args p, const int target) {
+__global__ __launch_bounds__(NW * 64, 2) void paged_attention_few_kernel(const estts_paged_attention_args p, const PagedCall c) {
     constexpr int ES = (int)sizeof(T), HALVES = tile_halves(DH, ES), TILE = 16 * HALVES;
     constexpr uint32_t ALL_ROWS = HALVES == 2 ? 0xFFFFFFFFu : 0xFFFFu;
     constexpr int NV = DH / 16, RUN = NV * ES < 16 ? NV : 16 / ES, RUNS = NV / RUN;        // features of a row per lane, of one load
@@ -843,14 +868,14 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_attention_few_kernel(const e
     __shared__ float m_s[NW][NQ], l_s[NW][NQ];
     const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const PagedUnit<NQ> u(p);
-    const PagedScratch ws(p.ws, target, p.H, DH);
+    const PagedUnit<NQ> u(p, c);
+    const PagedScratch ws(p.ws, c.target, p.H, DH);
     PagedPart<NW * 64, TILE * NW, SPLIT> part;
-    if (!part.find(p, u.part, target)) return;
+    if (!part.find(p, c, u.part)) return;
     do {
         const PagedSegment seg = part.next(p, u.h0 == 0 && threadIdx.x == 0 ? ws.items : nullptr);
         const int b = seg.b, begin = seg.begin, end = seg.end;
-        PageWalk<HALVES, NW> walk(p, b, begin, wave, ES);
+        PageWalk<HALVES, NW> walk(p, c, b, begin, wave, ES);
         const float qs = p.scale * 1.4426950408889634f;
         float qx[NQ][NV];
 #pragma unroll
@@ -1095,21 +1120,22 @@ extern "C" int64_t estts_page_plan_ws_bytes(int32_t B, int32_t T) {
 }
 
 template <bool PADDED, bool SPLIT>
-static void launch_page_scans(const estts_page_plan_args& a, hipStream_t st) {
-    if (a.B > PLAN_LDS) ESTTS_LAUNCH((page_plan_kernel<1024, false, PADDED, SPLIT>), dim3(1), dim3(1024), 0, st, a);
-    else if (a.B > 256 || (!SPLIT && a.T > 1024)) ESTTS_LAUNCH((page_plan_kernel<1024, true, PADDED, SPLIT>), dim3(1), dim3(1024), 0, st, a);
-    else ESTTS_LAUNCH((page_plan_kernel<256, true, PADDED, SPLIT>), dim3(1), dim3(256), 0, st, a);
+static void launch_page_scans(const estts_page_plan_args& a, const PageDivisors& by, hipStream_t st) {
+    if (a.B > PLAN_LDS) ESTTS_LAUNCH((page_plan_kernel<1024, false, PADDED, SPLIT>), dim3(1), dim3(1024), 0, st, a, by);
+    else if (a.B > 256 || (!SPLIT && a.T > 1024)) ESTTS_LAUNCH((page_plan_kernel<1024, true, PADDED, SPLIT>), dim3(1), dim3(1024), 0, st, a, by);
+    else ESTTS_LAUNCH((page_plan_kernel<256, true, PADDED, SPLIT>), dim3(1), dim3(256), 0, st, a, by);
 }
 
 template <bool PADDED>
 static void launch_page_plan(const estts_page_plan_args& a, hipStream_t st) {
-    if (a.T <= PLAN_ROWS) return launch_page_scans<PADDED, false>(a, st);
-    launch_page_scans<PADDED, true>(a, st);
+    const PageDivisors by = {page_size(a.page), divisor(PADDED ? a.R : 1, 30)};
+    if (a.T <= PLAN_ROWS) return launch_page_scans<PADDED, false>(a, by, st);
+    launch_page_scans<PADDED, true>(a, by, st);
     // (threads enough for the rows, for the pages that they may take and for those that may come back)
     const long wgs = ((long)a.T + a.T / a.page + a.B + a.n_pages + 255) / 256;
     const dim3 grid((unsigned)(wgs < 1024 ? wgs : 1024));
-    if (a.B > PLAN_LDS) ESTTS_LAUNCH((page_copy_kernel<false, PADDED>), grid, dim3(256), 0, st, a);
-    else ESTTS_LAUNCH((page_copy_kernel<true, PADDED>), grid, dim3(256), 0, st, a);
+    if (a.B > PLAN_LDS) ESTTS_LAUNCH((page_copy_kernel<false, PADDED>), grid, dim3(256), 0, st, a, by);
+    else ESTTS_LAUNCH((page_copy_kernel<true, PADDED>), grid, dim3(256), 0, st, a, by);
 }
 
 extern "C" int estts_page_plan(const estts_page_plan_args* args, void* stream) {
@@ -1178,12 +1204,13 @@ template <typename T, int DH, bool MASK, bool STREAM, bool SPLIT>
 static void launch_paged_attention(const estts_paged_attention_args& a, int target, hipStream_t stream) {
     const int group = a.H / a.kv_heads, n_group = (group + 15) / 16;
     const int units = (target ? target : a.B) * a.kv_heads;
+    const PagedCall c = {page_size(a.page), group, n_group, target, divisor(a.kv_heads, 30), divisor(target ? target : 1, 30)};
     const dim3 grid(n_group > 1 ? (units + 7) / 8 * 8 * n_group : units), block(ATT_WAVES * 64);
     constexpr int NW = SPLIT ? ATT_WAVES : FEW_WAVES;
     constexpr int FEW = few_queries((int)sizeof(T));
-    if (group == 1) ESTTS_LAUNCH((paged_attention_few_kernel<T, DH, MASK, STREAM, SPLIT, 1, NW>), grid, dim3(NW * 64), 0, stream, a, target);
-    else if (group <= FEW) ESTTS_LAUNCH((paged_attention_few_kernel<T, DH, MASK, STREAM, SPLIT, FEW, NW>), grid, dim3(NW * 64), 0, stream, a, target);
-    else ESTTS_LAUNCH((paged_attention_kernel<T, DH, MASK, STREAM, SPLIT, ATT_WAVES>), grid, block, 0, stream, a, target);
+    if (group == 1) ESTTS_LAUNCH((paged_attention_few_kernel<T, DH, MASK, STREAM, SPLIT, 1, NW>), grid, dim3(NW * 64), 0, stream, a, c);
+    else if (group <= FEW) ESTTS_LAUNCH((paged_attention_few_kernel<T, DH, MASK, STREAM, SPLIT, FEW, NW>), grid, dim3(NW * 64), 0, stream, a, c);
+    else ESTTS_LAUNCH((paged_attention_kernel<T, DH, MASK, STREAM, SPLIT, ATT_WAVES>), grid, block, 0, stream, a, c);
 }
 
 template <typename T, int DH, bool SPLIT>

@@ -157,6 +157,37 @@ def test_pages_must_be_a_multiple_of_sixteen_rows():
 
 # ------------------------------------------------------------------------------------------- models of the kernels' index arithmetic
 # The formulas restate csrc/paged.hip; a kernel change that moves an index has to move it here too.
+def divide(x, d, bits):
+    """Divisor: x / d for x below 2^bits, a product of 32-bit numbers and a shift."""
+    s = (d - 1).bit_length()
+    m = -(-(1 << (bits + s)) // d)
+    assert 0 < m < 2 ** 32 and bits + s < 64 and x < 2 ** bits
+    return x * m >> (bits + s)
+
+
+def pages(x, page):
+    """PageSize: x / page for x below 2^32."""
+    return divide(x >> 4, page // 16, 28)
+
+
+@pytest.mark.parametrize('bits', [28, 30])
+def test_divisions_are_exact(bits):
+    g = torch.Generator().manual_seed(bits)
+    ds = list(range(1, 70)) + [100, 127, 128, 129, 255, 256, 257, 1000, 4095, 4096, 65535, 2 ** 20 - 1, 2 ** 20 + 1, 2 ** 26, 2 ** bits - 1]
+    ds += torch.randint(1, 2 ** 24, (50,), generator=g).tolist()
+    for d in ds:
+        top = 2 ** bits - 1
+        xs = [0, 1, d - 1, d, d + 1, top, top - 1, top // d * d, max(top // d * d - 1, 0)] + torch.randint(0, 2 ** bits, (50,), generator=g).tolist()
+        xs += [k * d + e for k in (2, 3, top // d // 2) for e in (-1, 0, 1)]
+        for x in xs:
+            if 0 <= x <= top:
+                assert divide(x, d, bits) == x // d, (x, d)
+    for page in (16, 32, 48, 64, 112, 1600, 2 ** 30):
+        for x in (0, 1, page - 1, page, page + 1, 2 ** 31 - 1, 2 ** 31, 2 ** 32 - 1, 5 * page - 1, 5 * page):
+            if x < 2 ** 32:
+                assert pages(x, page) == x // page
+
+
 def request_rows(length, P, page, max_len):
     return min(max(length, 0), P * page, max_len)
 
@@ -167,13 +198,18 @@ def parts_of(lengths, target, unit):
     units = [max(-(-n // unit), 1) for n in lengths]
     total = sum(units)
     n_parts = min(target, total)
+    share = divide(total, target, 30) if total >= target else 1
+    extra = total - share * n_parts
+    part_of = lambda x: int(((x + 1.0) * n_parts - 1.0) / total)
     line, parts, items = 0, [], {}
     starts = []
     for n in units:
         starts.append(line)
         line += n
     for k in range(n_parts):
-        lo, hi = k * total // n_parts, (k + 1) * total // n_parts
+        lo = k * share + divide(k * extra, target, 30)
+        hi = lo + share + divide((k + 1) * extra, target, 30) - divide(k * extra, target, 30)
+        assert (lo, hi) == (k * total // n_parts, (k + 1) * total // n_parts)
         b = max(i for i, s in enumerate(starts) if s <= lo)
         off, left, at, segments = lo - starts[b], hi - lo, lo, []
         while left > 0:
@@ -181,7 +217,7 @@ def parts_of(lengths, target, unit):
             whole = take == units[b]
             segments.append((b, off, take, units[b], None if whole else 2 * k + (off == 0)))
             if off == 0:
-                items[b] = (k, 1 if whole else ((at + units[b]) * n_parts - 1) // total - k + 1)
+                items[b] = (k, 1 if whole else part_of(at + units[b] - 1) - k + 1)
             left, at, off, b = left - take, at + take, 0, b + 1
         parts.append(segments)
     return parts, items
