@@ -795,3 +795,70 @@ def test_scratch_goes_back_to_the_allocator():
                     ops.page_plan(lengths, new, table, free, n_free, 24, slots)
         torch.cuda.synchronize()
     assert torch.cuda.memory_allocated() == before
+
+
+# ------------------------------------------------------------------- the same conditions for every kernel: one, two, three queries a key head; cut or not
+EVERY_KERNEL = [pytest.mark.parametrize('kind', sorted(TYPES)), pytest.mark.parametrize('group', [1, 2, 3]), pytest.mark.parametrize('long', [False, True])]
+
+
+def every_kernel(test):
+    for mark in EVERY_KERNEL:
+        test = mark(test)
+    return test
+
+
+@every_kernel
+@pytest.mark.parametrize('D', [32, 128])
+def test_every_kernel_ignores_what_lies_in_masked_rows_and_behind_the_length(kind, group, long, D):
+    lengths = [70, 33, 2100 if long else 900, 16, 0, 129]
+    mask = torch.zeros(6, -(-max(lengths) // 16) * 16)
+    mask[:, 5::7] = 1.0
+    mask[2, 100:300] = float('nan')
+    mask[3] = torch.finfo(torch.float32).min          # nothing left
+
+    def spoil(table, kc, vc, m):
+        for c, bad in ((kc, float('inf')), (vc, float('nan'))):
+            for b, n in enumerate(lengths):
+                for pos in range(-(-n // 16) * 16):
+                    if pos >= n or m[b, pos] != 0:
+                        c[int(table[b, pos // 16]), :, pos % 16] = bad if pos % 2 else -float('inf')
+    got = check_attention(lengths, 2 * group, 2, D, 16, kind, mask=mask, spoil=spoil, seed=8)
+    assert bool((got[3:5] == 0).all())
+
+
+@every_kernel
+def test_every_kernel_leaves_out_pages_that_do_not_exist(kind, group, long):
+    def spoil(table, kc, vc, m):
+        table[0, 1], table[2, 0], table[2, 3], table[3, :] = -1, kc.shape[0], 2 ** 31 - 1, -2 ** 31
+    got = check_attention([100, 20, 2050 if long else 600, 64], 2 * group, 2, 64, 16, kind, spoil=spoil, seed=4)
+    assert bool((got[3] == 0).all())
+
+
+@every_kernel
+@pytest.mark.parametrize('order', ['token', 'gaps'])
+def test_every_kernel_takes_other_strides(kind, group, long, order):
+    check_attention([100, 37, 1600 if long else 400], 3 * group, 3, 64, 48, kind, order=order, seed=3)
+
+
+@every_kernel
+@pytest.mark.parametrize('scale,spread', [(-0.3, 1.0), (0.125, 1e-30), (2e-5, 3e4)])
+def test_every_kernel_takes_other_scales(kind, group, long, scale, spread):
+    check_attention([90, 1700 if long else 700], 2 * group, 2, 64, 16, kind, scale=scale, spread=spread, seed=9)
+
+
+@pytest.mark.parametrize('kind', ['bf16', 'f32'])
+@pytest.mark.parametrize('heads', [4, 16])
+def test_every_kernel_reaches_cache_offsets_past_32_bits(kind, heads):
+    Hk, D, page = 4, 128, 64
+    n_pages = (1 << 32) // (Hk * D * page) + 40
+    kc, vc = (torch.empty(n_pages, Hk, page, D, dtype=TYPES[kind], device=DEV) for _ in range(2))
+    ids = [n_pages - 1, 3, n_pages - 30, n_pages // 2 + 1, n_pages - 2, 7]
+    g = torch.Generator(device=DEV).manual_seed(1)
+    rows = torch.randn(6 * page, Hk * D, generator=g, device=DEV)
+    ops.page_write(rows, rows.flip(0), kc, vc, torch.cat([torch.arange(i * page, (i + 1) * page) for i in ids]).int().to(DEV))
+    q = torch.randn(2, heads * D, generator=g, device=DEV)
+    small = [c[torch.tensor(ids, device=DEV)].contiguous() for c in (kc, vc)]
+    outs = [ops.paged_attention(q, *c, torch.tensor(t, dtype=torch.int32).view(2, 3).to(DEV), dev([150, 192]), torch.empty_like(q), heads)
+            for c, t in (((kc, vc), ids), (small, list(range(6))))]
+    want, bound = attention_oracle(q.cpu(), small[0].cpu(), small[1].cpu(), torch.arange(6).view(2, 3), [150, 192], heads, None, 1 / math.sqrt(D), 192)
+    assert torch.equal(*outs) and bool(((outs[0].cpu().double() - want).abs() <= bound).all())
