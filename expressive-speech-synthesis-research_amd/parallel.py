@@ -74,8 +74,8 @@ def _staged(t, group=None):
 def all_reduce_sum_(t, group=None):
     """In-place sum of `t` over all ranks, blocking.  Over gloo a device tensor goes through a host copy made HERE and the
     host tensor is what gloo sees: ProcessGroupGloo's own device path (staging threads and streams of its own) has stalled for
-    good with two processes on one GPU -- two collectives in flight behind queued kernels at first
-    (tools/gloo_concurrent.py), later a single one, both ranks inside the same all-reduce with two of gloo's threads in an
+    good with two processes on one GPU -- two collectives in flight behind queued kernels at first,
+    later a single one, both ranks inside the same all-reduce with two of gloo's threads in an
     uninterruptible driver call -- and the rehearsal transport is not what is being rehearsed."""
     if _staged(t, group):
         h = t.detach().to('cpu')
@@ -145,8 +145,7 @@ class GradientOverlap:
         # gloo stages device buffers through host threads of its own; collectives issued while kernels are still queued
         # stalled two ranks sharing one GPU, so with gloo on device memory the whole exchange waits for finish() and then
         # goes out bucket by bucket through host copies made here
-        self.defer = (self.active and flat.is_cuda and dist.get_backend(group) != 'nccl'
-                      and os.environ.get('ESTTS_GLOO_OVERLAP', '0') != '1')     # (diagnostic switch: overlap over gloo anyway)
+        self.defer = self.active and _staged(flat, group)
         self.final = False
         self.hi = flat.numel()
         self.works = []

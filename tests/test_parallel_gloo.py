@@ -104,3 +104,26 @@ def test_bench_gpus_flag_starts_the_ranks_itself():
     r = subprocess.run([sys.executable, os.path.join(root, 'bench.py'), '--gpus', '2', '--workload', 'exchange', '--elems', '1000',
                         '--steps', '1', '--warmup', '0'], capture_output=True, text=True, timeout=120, env=env2, cwd=root)
     assert r.returncode != 0 and '--gpus 2' in (r.stderr + r.stdout)
+
+
+class _OnDevice:
+    """What GradientOverlap asks of a flat buffer when it is made, as a device tensor answers."""
+    is_cuda = True
+
+    def numel(self):
+        return 1003
+
+
+def test_a_device_buffer_over_gloo_is_never_exchanged_during_the_backward_pass(monkeypatch):
+    """Collectives that gloo would run on device tensors behind queued kernels have hung: nothing turns that order on again."""
+    monkeypatch.setattr(parallel.dist, 'is_initialized', lambda: True)
+    monkeypatch.setattr(parallel.dist, 'get_world_size', lambda group=None: 2)
+    monkeypatch.setenv('ESTTS_GLOO_OVERLAP', '1')
+    for backend, held in (('gloo', True), ('nccl', False)):
+        monkeypatch.setattr(parallel.dist, 'get_backend', lambda group=None: backend)
+        overlap = parallel.GradientOverlap(_OnDevice(), 250)
+        assert overlap.defer is held
+    monkeypatch.setattr(parallel.dist, 'get_backend', lambda group=None: 'gloo')
+    overlap = parallel.GradientOverlap(_OnDevice(), 250)
+    overlap.ready(100)
+    assert overlap.calls == [] and overlap.works == []
