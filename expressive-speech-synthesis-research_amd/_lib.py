@@ -324,7 +324,7 @@ def load_host():
         at = [C.cast(getattr(lib, n), _vp).value for n in ('estts_page_plan', 'estts_page_write', 'estts_paged_attention', 'estts_page_plan_ws_bytes',
                                                            'estts_paged_attention_ws_bytes')]
         mod.setup(*at, torch._C._cuda_cudaCachingAllocator_raw_alloc, torch._C._cuda_cudaCachingAllocator_raw_delete, torch._C._cuda_getDevice,
-                  torch._C._cuda_getCurrentRawStream)
+                  torch._C._cuda_getCurrentRawStream, lambda what: check(-2, what))
         _host = mod
     return _host
 

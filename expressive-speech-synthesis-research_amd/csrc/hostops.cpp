@@ -4,9 +4,10 @@
  * asked for the tensors' attributes through Python; 4.1 here).
  *
  * Every function returns True if it has issued the launch, and False, with nothing done and no error set, if anything at all is out of the
- * ordinary: a type, shape, stride or device that is not what the operator takes, a tensor subclass, or an error of the C ABI.  The
+ * ordinary: a type, shape, stride or device that is not what the operator takes, a tensor subclass, or a call that the C ABI refuses.  The
  * caller then takes the Python path, whose checks say what is wrong.  So there is one place for messages, and this file only has to
- * accept nothing that ops.py would refuse. */
+ * accept nothing that ops.py would refuse.  An error of the runtime (the C ABI's -2) raises instead: the launch may be under way all the
+ * same (the error can be one that an earlier call of another library left behind), and a plan issued twice plans its rows twice. */
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 #include <math.h>
@@ -24,7 +25,7 @@ struct {
     int (*attention)(const estts_paged_attention_args*, void*);
     int64_t (*plan_ws)(int32_t, int32_t);
     int64_t (*attention_ws)(int32_t, int32_t, int32_t, int32_t, int32_t, int32_t);
-    PyObject *alloc, *free, *get_device, *get_stream;
+    PyObject *alloc, *free, *get_device, *get_stream, *fail;
 } host;
 
 const at::ScalarType KV_TYPES[3] = {at::kFloat, at::kBFloat16, at::kHalf};      // ESTTS_KV_*
@@ -151,19 +152,22 @@ struct Scratch {
     }
 };
 
+// What became of a call.  (false is TURNED_DOWN)
+enum { TURNED_DOWN = 0, ISSUED = 1, FAILED = 2 };
+
 // Issues a launch without the interpreter's lock: it waits where the stream's queue is full.
 template <typename A>
-bool launch(int (*f)(const A*, void*), const A& args, void* stream) {
+int launch(int (*f)(const A*, void*), const A& args, void* stream) {
     PyThreadState* state = PyEval_SaveThread();
     const int rc = f(&args, stream);
     PyEval_RestoreThread(state);
-    return rc == 0;
+    return rc == 0 ? ISSUED : rc == -1 ? TURNED_DOWN : FAILED;
 }
 
 bool fits32(int64_t x) { return x >= 0 && x <= INT32_MAX; }
 
 // page_write(k, v, k_cache, v_cache, slots)
-bool page_write(PyObject* const* a, Py_ssize_t n) {
+int page_write(PyObject* const* a, Py_ssize_t n) {
     tensor k, v, kc, vc, slots;
     estts_page_write_args w;
     void* stream;
@@ -180,7 +184,7 @@ bool page_write(PyObject* const* a, Py_ssize_t n) {
 }
 
 // page_plan(lengths, new, block_table, free_pages, n_free, page, slots, positions, lengths_out, n_free_out, refused)
-bool page_plan(PyObject* const* a, Py_ssize_t n) {
+int page_plan(PyObject* const* a, Py_ssize_t n) {
     tensor lengths, news, table, pages, n_free, slots, positions, lengths_out, n_free_out, refused;
     estts_page_plan_args w;
     int64_t page;
@@ -212,7 +216,7 @@ bool page_plan(PyObject* const* a, Py_ssize_t n) {
 }
 
 // paged_attention(q, k_cache, v_cache, block_table, lengths, ctx, heads, key_mask, scale, max_len)
-bool paged_attention(PyObject* const* a, Py_ssize_t n) {
+int paged_attention(PyObject* const* a, Py_ssize_t n) {
     tensor q, kc, vc, table, lengths, ctx, mask;
     estts_paged_attention_args w;
     int64_t heads, max_len;
@@ -250,35 +254,40 @@ bool paged_attention(PyObject* const* a, Py_ssize_t n) {
 }
 
 // (a tensor that only looks plain, of a function transform, say, throws when its address is asked for)
-template <bool (*F)(PyObject* const*, Py_ssize_t)>
+const char* const NAMES[3] = {"estts_page_plan", "estts_page_write", "estts_paged_attention"};
+
+template <int (*F)(PyObject* const*, Py_ssize_t), int NAME>
 PyObject* entry(PyObject*, PyObject* const* a, Py_ssize_t n) {
-    bool issued = false;
-    try { issued = F(a, n); } catch (...) {}
-    return PyBool_FromLong(issued);
+    int answer = TURNED_DOWN;
+    try { answer = F(a, n); } catch (...) {}
+    if (answer != FAILED) return PyBool_FromLong(answer);
+    Py_XDECREF(PyObject_CallFunction(host.fail, "s", NAMES[NAME]));
+    if (!PyErr_Occurred()) PyErr_Format(PyExc_RuntimeError, "%s failed", NAMES[NAME]);
+    return nullptr;
 }
 
 // setup(addresses of estts_page_plan, _page_write, _paged_attention, _page_plan_ws_bytes, _paged_attention_ws_bytes, allocate (bytes, stream),
-// free (address), current device (), raw stream (device))
+// free (address), current device (), raw stream (device), raise the library's last error of an entry point (its name))
 PyObject* setup(PyObject*, PyObject* const* a, Py_ssize_t n) {
     int64_t f[5];
-    if (n != 9) { PyErr_SetString(PyExc_TypeError, "setup takes 9 arguments"); return nullptr; }
+    if (n != 10) { PyErr_SetString(PyExc_TypeError, "setup takes 10 arguments"); return nullptr; }
     for (int i = 0; i < 5; ++i)
         if (!as_int(a[i], f + i) || !f[i]) { PyErr_SetString(PyExc_TypeError, "setup: addresses must be non-zero integers"); return nullptr; }
-    for (int i = 5; i < 9; ++i) Py_INCREF(a[i]);
+    for (int i = 5; i < 10; ++i) Py_INCREF(a[i]);
     host.plan = reinterpret_cast<decltype(host.plan)>(f[0]);
     host.write = reinterpret_cast<decltype(host.write)>(f[1]);
     host.attention = reinterpret_cast<decltype(host.attention)>(f[2]);
     host.plan_ws = reinterpret_cast<decltype(host.plan_ws)>(f[3]);
     host.attention_ws = reinterpret_cast<decltype(host.attention_ws)>(f[4]);
-    host.alloc = a[5]; host.free = a[6]; host.get_device = a[7]; host.get_stream = a[8];
+    host.alloc = a[5]; host.free = a[6]; host.get_device = a[7]; host.get_stream = a[8]; host.fail = a[9];
     Py_RETURN_NONE;
 }
 
 template <typename F>
 PyMethodDef method(const char* name, F f) { return {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL, nullptr}; }
 
-PyMethodDef methods[] = {method("setup", setup), method("page_plan", entry<page_plan>), method("page_write", entry<page_write>),
-                         method("paged_attention", entry<paged_attention>), {nullptr, nullptr, 0, nullptr}};
+PyMethodDef methods[] = {method("setup", setup), method("page_plan", entry<page_plan, 0>), method("page_write", entry<page_write, 1>),
+                         method("paged_attention", entry<paged_attention, 2>), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_hostops", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -1,5 +1,6 @@
 """Paged decoding on the GPU (estts_page_plan, estts_page_write, estts_paged_attention) against plain restatements: the plan in whole
 numbers, the write bit for bit, the attention in float64 with bounds derived from the arithmetic (see attention_bound)."""
+import ctypes
 import math
 
 import pytest
@@ -862,3 +863,45 @@ def test_every_kernel_reaches_cache_offsets_past_32_bits(kind, heads):
             for c, t in (((kc, vc), ids), (small, list(range(6))))]
     want, bound = attention_oracle(q.cpu(), small[0].cpu(), small[1].cpu(), torch.arange(6).view(2, 3), [150, 192], heads, None, 1 / math.sqrt(D), 192)
     assert torch.equal(*outs) and bool(((outs[0].cpu().double() - want).abs() <= bound).all())
+
+
+# ------------------------------------------------------------------------------------------------------- launches that fail
+def test_a_launch_that_fails_is_issued_once_and_said(monkeypatch):
+    """The C++ module's entry points answer -2 (an error of the runtime, the launch possibly under way): the call raises, and is not issued
+    again by the Python path, which would plan the same rows twice.  -1 (refused, nothing issued) goes to the Python path as ever."""
+    lib, calls, answer = ops._lib, [], [-2]
+    entry = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p)
+    names = ('estts_page_plan', 'estts_page_write', 'estts_paged_attention')
+
+    def said(name):
+        def f(args, stream):
+            calls.append(name)
+            return answer[0]
+        return entry(f)
+    fakes = {n: said(n) for n in names}
+    loop = Loop('f32')
+    loop.new.fill_(1)
+    H, Hk, D = loop.H, loop.Hk, loop.D
+    k, v = loop.qkv[:, H * D:(H + Hk) * D], loop.qkv[:, (H + Hk) * D:]
+    plan = lambda: ops.page_plan(loop.lengths, loop.new, loop.table, loop.free, loop.n_free, loop.page, loop.slots)
+    write = lambda: ops.page_write(k, v, loop.kc, loop.vc, loop.slots)
+    attend = lambda: ops.paged_attention(loop.qkv[:, :H * D], loop.kc, loop.vc, loop.table, loop.lengths, loop.ctx, H)
+    plan()
+    try:
+        with monkeypatch.context() as mp:               # (only the C++ module's addresses: the Python path keeps the library's)
+            for n in names:
+                mp.setattr(lib.load(), n, fakes[n])
+            lib._host = None
+            lib.load_host()
+        for call in (plan, write, attend):
+            with pytest.raises(lib.EsttsError):
+                call()
+        assert calls == list(names) and loop.lengths.tolist() == [1] * loop.B
+        answer[0] = -1
+        plan()
+        assert loop.lengths.tolist() == [2] * loop.B
+    finally:
+        lib._host = None
+        lib.load_host()
+    plan()
+    assert loop.lengths.tolist() == [3] * loop.B and len(calls) == 4
