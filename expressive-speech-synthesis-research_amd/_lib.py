@@ -6,6 +6,7 @@ symbol, importing an op raises.  Build it with `make -C <package>/csrc` (or
 """
 import ctypes as C
 import os
+import warnings
 
 _PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG, 'libestts.so')
@@ -304,23 +305,30 @@ def load():
     return lib
 
 
-_host = None
+_host = None        # the C++ module, False where it cannot be used
 
 
 def load_host():
     """The C++ module that issues the paged-decoding operators (csrc/hostops.cpp), set up with this library's entry points and torch's
-    allocator, device and stream queries; raise if it is not built."""
+    allocator, device and stream queries.  False, with one warning, if it is not built, not loadable or built against another torch or
+    C ABI: the operators then issue the same launches from Python, some 4 us a call later."""
     global _host
     if _host is None:
         lib = load()
         import torch
         from importlib import machinery, util
         path = os.path.join(_PKG, '_hostops.so')
-        if not os.path.exists(path):
-            raise EsttsError(f'{path} not found: the extension is not built (make -C {_PKG}/csrc)')
         spec = util.spec_from_file_location('_hostops', path, loader=machinery.ExtensionFileLoader('_hostops', path))
-        mod = util.module_from_spec(spec)
-        spec.loader.exec_module(mod)
+        try:
+            mod = util.module_from_spec(spec)
+            spec.loader.exec_module(mod)
+            if mod.built_for != (str(torch.__version__), ABI_VERSION):
+                raise ImportError(f'built for torch {mod.built_for[0]} and ABI version {mod.built_for[1]}, found {torch.__version__} and {ABI_VERSION}')
+        except (ImportError, AttributeError) as e:
+            warnings.warn(f'{path} is not used, paged decoding issues its launches from Python ({e}); build it with make -C {_PKG}/csrc',
+                          RuntimeWarning, stacklevel=2)
+            _host = False
+            return _host
         at = [C.cast(getattr(lib, n), _vp).value for n in ('estts_page_plan', 'estts_page_write', 'estts_paged_attention', 'estts_page_plan_ws_bytes',
                                                            'estts_paged_attention_ws_bytes')]
         mod.setup(*at, torch._C._cuda_cudaCachingAllocator_raw_alloc, torch._C._cuda_cudaCachingAllocator_raw_delete, torch._C._cuda_getDevice,

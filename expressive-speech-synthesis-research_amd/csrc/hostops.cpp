@@ -292,4 +292,12 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_hostops", nullptr, -1, methods, n
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__hostops(void) { return PyModule_Create(&module); }
+// built_for: the torch whose headers this was compiled against and the C ABI of estts.h, for the loader to compare
+PyMODINIT_FUNC PyInit__hostops(void) {
+    PyObject* m = PyModule_Create(&module);
+    PyObject* built_for = m ? Py_BuildValue("(si)", ESTTS_TORCH, ESTTS_ABI_VERSION) : nullptr;
+    if (built_for && PyModule_AddObject(m, "built_for", built_for) == 0) return m;
+    Py_XDECREF(built_for);
+    Py_XDECREF(m);
+    return nullptr;
+}

@@ -691,11 +691,11 @@ def _check_pages(what, k_cache, v_cache):
 
 
 def _issue():
-    """The C++ module that issues plain calls of the operators below, None while launches are recorded, traced or named: those, and whatever
-    the module turns down, take the Python path behind it, which says what is wrong."""
+    """The C++ module that issues plain calls of the operators below, None while launches are recorded, traced or named and where the module is
+    not built for this torch: those, and whatever the module turns down, take the Python path behind it, which says what is wrong."""
     if _program is not None or _trace is not None or _debug_sync:
         return None
-    return _lib._host or _lib.load_host()
+    return (_lib.load_host() if _lib._host is None else _lib._host) or None
 
 
 def new_paged_cache(n_pages, page, kv_heads, depth, dtype=torch.float32, device='cuda'):

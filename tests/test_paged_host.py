@@ -3,6 +3,7 @@ CPU tensors), the layout of the argument blocks, and models of the kernels' inde
 import ctypes
 import os
 import subprocess
+import warnings
 
 import pytest
 import torch
@@ -318,3 +319,32 @@ def test_which_calls_are_cut(B, heads, kv_heads, depth, max_len, type, cut):
     nbytes = lib.estts_paged_attention_ws_bytes(B, heads, kv_heads, depth, max_len, type)
     parts = max(1, 256 // (kv_heads * -(-heads // kv_heads // 16)))
     assert nbytes == (2 * parts * heads * (depth + 2) * 4 + 8 * B if cut else 0)
+
+
+# -------------------------------------------------------------------------------------------------------------- the C++ module
+def test_the_cpp_module_is_built_for_this_torch():
+    assert _lib.load_host() and _lib.load_host().built_for == (torch.__version__, _lib.ABI_VERSION)
+
+
+@pytest.mark.parametrize('why', ['missing', 'not a module', 'another torch', 'another ABI', 'an older build'])
+def test_without_a_usable_cpp_module_calls_take_the_python_path(monkeypatch, tmp_path, why):
+    """Said once, not raised: the kernels are all there without it."""
+    real = _lib.load_host()
+    monkeypatch.setattr(_lib, '_host', None)
+    if why in ('missing', 'not a module'):
+        monkeypatch.setattr(_lib, '_PKG', str(tmp_path))
+        if why == 'not a module':
+            (tmp_path / '_hostops.so').write_bytes(b'no library')
+    elif why == 'an older build':
+        monkeypatch.delattr(real, 'built_for')
+        monkeypatch.setattr('importlib.util.module_from_spec', lambda spec: real)
+        monkeypatch.setattr('importlib.machinery.ExtensionFileLoader.exec_module', lambda self, mod: None)
+    else:
+        monkeypatch.setattr(*((torch, '__version__', '1.0') if why == 'another torch' else (_lib, 'ABI_VERSION', 0)))
+    with pytest.warns(RuntimeWarning, match='from Python'):
+        assert ops._issue() is None
+    with warnings.catch_warnings():
+        warnings.simplefilter('error')
+        assert ops._issue() is None and _lib._host is False
+        with pytest.raises((ValueError, TypeError)):                # (the Python path, and its checks)
+            ops.paged_attention(*[torch.zeros(1)] * 6, 1)
