@@ -321,6 +321,51 @@ def test_which_calls_are_cut(B, heads, kv_heads, depth, max_len, type, cut):
     assert nbytes == (2 * parts * heads * (depth + 2) * 4 + 8 * B if cut else 0)
 
 
+# ---------------------------------------------------------------------------------- where the kernels' addresses lie, bad ids among them
+def half_at(entry, r, page, n_pages, max_len, s_page, s_row):
+    """PageWalk: the byte (here: element) offset of the sixteen rows from r on in a page named `entry`, through place()'s two 32-bit halves and
+    locate(); (offset, whether they count)."""
+    there = entry >= 0 and entry < n_pages and r < max_len
+    x = entry * s_page + (r - r // page * page) * s_row if there else -1
+    lo, hi = x & 0xFFFFFFFF, (x >> 32) & 0xFFFFFFFF
+    hi -= (hi & 0x80000000) << 1
+    return ((hi & 0xFFFFFFFF) << 32 | lo, True) if hi >= 0 else (0, False)
+
+
+def slot_at(slot, h, page, n_pages, s_page, s_head, s_row):
+    """page_write_kernel: the element a row's head goes to, or None."""
+    slot &= 0xFFFFFFFF
+    return None if slot >= n_pages * page else slot // page * s_page + h * s_head + slot % page * s_row
+
+
+STRIDES = {'head': lambda Hk, page, D: (Hk * page * D, page * D, D), 'token': lambda Hk, page, D: (page * Hk * D, D, Hk * D),
+           'gaps': lambda Hk, page, D: ((Hk + 1) * (page + 3) * (D + 16), (page + 3) * (D + 16), D + 16)}
+
+
+@pytest.mark.parametrize('order', sorted(STRIDES))
+@pytest.mark.parametrize('n_pages,page,Hk,D', [(1, 16, 1, 32), (7, 16, 3, 64), (7, 48, 2, 128), (131113, 64, 4, 128)])
+def test_addresses_lie_in_the_cache_or_are_not_taken(n_pages, page, Hk, D, order):
+    """Every id and slot, those at and past the ends of the cache among them: what the attention loads is sixteen rows that the cache has
+    (row 0 of page 0 in the place of rows that do not count), what the write stores is a row that it has; valid ones are all taken."""
+    s_page, s_head, s_row = STRIDES[order](Hk, page, D)
+    end = (n_pages - 1) * s_page + (Hk - 1) * s_head + (page - 1) * s_row + D           # one past the last element
+    heads = (0, Hk - 1)
+    max_len = 5 * page - 7
+    for entry in (-2 ** 31, -n_pages, -1, 0, 1, n_pages // 2, n_pages - 1, n_pages, n_pages + 1, 2 ** 31 - 1):
+        for r in list(range(0, 5 * page, 16)) + [5 * page, 1 << 30]:
+            at, counts = half_at(entry, r, page, n_pages, max_len, s_page, s_row)
+            assert counts == (0 <= entry < n_pages and r < max_len)
+            assert at == (entry * s_page + r % page * s_row if counts else 0)
+            for h in heads:
+                assert 0 <= at + h * s_head and at + h * s_head + 15 * s_row + D <= end
+    total = n_pages * page
+    for slot in (-2 ** 31, -total, -page, -1, 0, 1, page - 1, page, total // 2, total - page, total - 1, total, total + 1, 2 ** 31 - 1):
+        for h in heads:
+            at = slot_at(slot, h, page, n_pages, s_page, s_head, s_row)
+            assert (at is not None) == (0 <= slot < total)
+            assert at is None or (0 <= at and at + D <= end and at == slot // page * s_page + h * s_head + slot % page * s_row)
+
+
 # -------------------------------------------------------------------------------------------------------------- the C++ module
 def test_the_cpp_module_is_built_for_this_torch():
     assert _lib.load_host() and _lib.load_host().built_for == (torch.__version__, _lib.ABI_VERSION)
