@@ -905,3 +905,26 @@ def test_a_launch_that_fails_is_issued_once_and_said(monkeypatch):
         lib.load_host()
     plan()
     assert loop.lengths.tolist() == [3] * loop.B and len(calls) == 4
+
+
+# ------------------------------------------------------------------------------------------------ small values, bounded by themselves
+@pytest.mark.parametrize('kind,scale_of', [('f16', 1e-6), ('f16', 2e4), ('bf16', 1e-30), ('bf16', 1e30), ('f32', 1e-30), ('f32', 1e30)])
+@pytest.mark.parametrize('heads', [2, 4, 6])
+@pytest.mark.parametrize('lengths', [[90, 700], [90, 1400]])
+def test_attention_of_very_small_and_very_large_values(kind, scale_of, heads, lengths):
+    """attention_bound without its absolute term, which is as large as outputs of 1e-30 are themselves.  In its place what can be lost where a
+    product or a piece is below the smallest normal number: each of a row's at most three pieces and its product less than 2^-126, so
+    (3 + 1) n 2^-126, 4e-35 at 700 rows where the outputs are some 4e-32.  Zeros in place of the outputs are out of these bounds."""
+    g = torch.Generator().manual_seed(heads)
+    table, n_pages = pages_for(lengths, 16, g)
+    kc, vc = cache_pair(n_pages, 16, 2, 64, torch.float32, seed=5)
+    most = torch.finfo(TYPES[kind]).max
+    kc, vc = ((c * scale_of).clamp(-most, most).to(TYPES[kind]) for c in (kc, vc))
+    q = torch.randn(2, heads * 64, generator=g)
+    scale = 0.1 / scale_of if scale_of < 1e20 else 1e-31
+    ctx = torch.full((2, heads * 64), 9.0, device=DEV)
+    ops.paged_attention(q.to(DEV), kc, vc, table.to(DEV), dev(lengths), ctx, heads, scale=scale)
+    want, bound = attention_oracle(q, kc.cpu(), vc.cpu(), table, lengths, heads, None, scale, table.shape[1] * 16)
+    bound = (bound - 1e-30) + 4 * torch.tensor(lengths)[:, None] * 2.0 ** -126
+    assert bool((want.abs().view(2, heads, 64).amax(-1) > 20 * bound.view(2, heads, 64).amax(-1)).all())
+    assert bool(((ctx.cpu().double() - want).abs() <= bound).all())
