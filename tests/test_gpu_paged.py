@@ -928,3 +928,17 @@ def test_attention_of_very_small_and_very_large_values(kind, scale_of, heads, le
     bound = (bound - 1e-30) + 4 * torch.tensor(lengths)[:, None] * 2.0 ** -126
     assert bool((want.abs().view(2, heads, 64).amax(-1) > 20 * bound.view(2, heads, 64).amax(-1)).all())
     assert bool(((ctx.cpu().double() - want).abs() <= bound).all())
+
+
+@pytest.mark.parametrize('layout', ['packed', 'padded'])
+def test_page_plan_where_requests_without_need_follow_refused_ones(layout):
+    """The height of the stack goes down by the pages that were taken, not by what refused requests had asked for: requests that take a page, ask
+    for more than there are, have room in their last page, end, have room, ask for more than there are."""
+    lengths, new = [16, 16, 5, 40, 17, 16], [3, 40, 1, -1, 2, 200]
+    table, free, n_free = [[0] + [-1] * 13, [1] + [-1] * 13, [2] + [-1] * 13, [3, 4, 5] + [-1] * 11, [6, 7] + [-1] * 12, [8] + [-1] * 13], list(range(9, 12)) + [-9] * 9, 3
+    size = dict(T=300) if layout == 'packed' else dict(R=200)
+    for stack in (3, 0):                             # (the one that ends gives three back)
+        want = plan_oracle(lengths, new, table, free, stack, 16, **size)
+        assert run_plan(lengths, new, table, free, stack, 16, **size) == want and want['n_free'] == 2
+    got = run_plan([16, 16, 5], [3, 60, 1], table[:3], free, 3, 16, **(dict(T=64) if layout == 'packed' else dict(R=60)))
+    assert got['n_free'] == 2 and got['refused'] == 1 and got['lengths'] == [19, 16, 6]
