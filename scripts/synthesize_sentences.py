@@ -28,19 +28,55 @@ from estts.config_manager import ConfigManager  # noqa: E402
 from estts.synthesizer_wavernn import Synthesize  # noqa: E402
 
 
-def synthesize_file(args, model):
+def conditioning(args, cm):
+    """(reference mel, speaker embedding) that the autoregressive model's system_type asks for, None for the others."""
+    ref = np.load(args.ref_mel) if args.ref_mel else None
+    if args.ref_wav:
+        import wave
+        from estts.audio import Audio
+        with wave.open(args.ref_wav, 'rb') as f:
+            if f.getsampwidth() != 2 or f.getnchannels() != 1 or f.getframerate() != cm.config['sampling_rate']:
+                raise SystemExit(f'--ref-wav must be 16-bit mono at {cm.config["sampling_rate"]} Hz')
+            pcm = np.frombuffer(f.readframes(f.getnframes()), dtype='<i2').astype(np.float32) / 32768.0
+        ref = Audio(cm.config).mel_spectrogram(pcm).t().contiguous()           # (T, 80), stays on the device
+    system = cm.config['system_type']
+    if 'style' in system and ref is None:
+        raise SystemExit(f"system_type '{system}' needs --ref-mel or --ref-wav")
+    spk = None
+    if 'speaker' in system:
+        if not args.spk_embed:
+            raise SystemExit(f"system_type '{system}' needs --spk-embed")
+        spk = np.load(args.spk_embed).astype(np.float32).reshape(1, -1)
+        n_spk = cm.model_config_dict()['speaker_embed_dim']
+        if spk.shape[1] != n_spk:
+            raise SystemExit(f'--spk-embed has {spk.shape[1]} values, the model expects {n_spk}')
+    return ref if 'style' in system else None, spk
+
+
+def synthesize_file(args, cm, model):
     """The reference's loop over sentences (synthesize_sentences_speaker.py:56-75) with the sentences overlapped: the forward
-    model keeps --in-flight of them on the GPU at once, and WaveRNN takes every fold of every utterance as one batch."""
-    if args.model != 'forward':
-        raise SystemExit('--text-file runs the forward model (the autoregressive model synthesises one sentence per call)')
+    model keeps --in-flight of them on the GPU at once, the autoregressive model decodes that many side by side out of paged caches, and
+    WaveRNN takes every fold of every utterance as one batch."""
     with open(args.text_file) as f:
         texts = [line.strip() for line in f if line.strip()]
     hp = configs.wavernn_hparams()
     vocoder = Synthesize(args.vocoder_weights, hp)
-    model.predict_many(texts[:args.in_flight], in_flight=args.in_flight)          # library load, workspaces, first-visit shapes
+    if args.model == 'forward':
+        predict = lambda texts: model.predict_many(texts, in_flight=args.in_flight)
+    else:
+        ref, spk = conditioning(args, cm)
+
+        def predict(texts):
+            outs = []
+            for i in range(0, len(texts), args.in_flight):
+                part = texts[i:i + args.in_flight]
+                outs += model.predict_many(part, None if ref is None else [ref] * len(part), None if spk is None else [spk] * len(part),
+                                           max_length=args.max_length)
+            return outs
+    predict(texts[:args.in_flight])                                               # library load, workspaces, first-visit shapes
     torch.cuda.synchronize()
     t0 = time.perf_counter()
-    outs = model.predict_many(texts, in_flight=args.in_flight)
+    outs = predict(texts)
     torch.cuda.synchronize()
     t_tts = time.perf_counter() - t0
     frames = sum(int(o['mel'].shape[0]) for o in outs)
@@ -63,10 +99,10 @@ def main():
     ap.add_argument('--config', required=True)
     ap.add_argument('--model', default='forward', choices=['forward', 'autoregressive'])
     ap.add_argument('--text')
-    ap.add_argument('--text-file', help='one sentence (phonemes) per line: all of them are synthesised, --in-flight at a time by the '
-                                        'forward model, and vocoded in one batched WaveRNN generation; outputs <out stem>_<i>.npy')
-    ap.add_argument('--in-flight', type=int, default=4, help='sentences the forward model keeps on the GPU at once with --text-file '
-                                                             '(ForwardTransformer.predict_many; 1 = one at a time)')
+    ap.add_argument('--text-file', help='one sentence (phonemes) per line: all of them are synthesised, --in-flight at a time, and vocoded in '
+                                        'one batched WaveRNN generation; outputs <out stem>_<i>.npy')
+    ap.add_argument('--in-flight', type=int, help='sentences on the GPU at once with --text-file (predict_many of either model; 1 = one at a time; '
+                                                  'default 4 for the forward model, 32 for the autoregressive one)')
     ap.add_argument('--tts-weights')
     ap.add_argument('--vocoder-weights')
     ap.add_argument('--ref-mel', help='.npy reference mel (T, 80) for the style encoder (autoregressive model)')
@@ -81,37 +117,22 @@ def main():
     args = ap.parse_args()
     if not args.text and not args.text_file:
         ap.error('give --text or --text-file')
+    if args.in_flight is None:
+        args.in_flight = 4 if args.model == 'forward' else 32
+    if args.in_flight < 1:
+        ap.error('--in-flight must be positive')
     cm = ConfigManager(args.config, args.model)
     if args.system_type:
         cm.config['system_type'] = args.system_type
     model = cm.load_model(args.tts_weights, verbose=True)
     if args.text_file:
-        return synthesize_file(args, model)
+        return synthesize_file(args, cm, model)
     t0 = time.perf_counter()
     if args.model == 'forward':
         out = model.predict(args.text)
     else:
-        ref = np.load(args.ref_mel) if args.ref_mel else None
-        if args.ref_wav:
-            import wave
-            from estts.audio import Audio
-            with wave.open(args.ref_wav, 'rb') as f:
-                if f.getsampwidth() != 2 or f.getnchannels() != 1 or f.getframerate() != cm.config['sampling_rate']:
-                    raise SystemExit(f'--ref-wav must be 16-bit mono at {cm.config["sampling_rate"]} Hz')
-                pcm = np.frombuffer(f.readframes(f.getnframes()), dtype='<i2').astype(np.float32) / 32768.0
-            ref = Audio(cm.config).mel_spectrogram(pcm).t().contiguous()           # (T, 80), stays on the device
-        system = cm.config['system_type']
-        if 'style' in system and ref is None:
-            raise SystemExit(f"system_type '{system}' needs --ref-mel or --ref-wav")
-        spk = None
-        if 'speaker' in system:
-            if not args.spk_embed:
-                raise SystemExit(f"system_type '{system}' needs --spk-embed")
-            spk = np.load(args.spk_embed).astype(np.float32).reshape(1, -1)
-            n_spk = cm.model_config_dict()['speaker_embed_dim']
-            if spk.shape[1] != n_spk:
-                raise SystemExit(f'--spk-embed has {spk.shape[1]} values, the model expects {n_spk}')
-        out = model.predict(args.text, ref if 'style' in system else None, spk, max_length=args.max_length, verbose=False)
+        ref, spk = conditioning(args, cm)
+        out = model.predict(args.text, ref, spk, max_length=args.max_length, verbose=False)
     mel = out['mel']
     hp = configs.wavernn_hparams()
     vocoder = Synthesize(args.vocoder_weights, hp)             # synthesize_sentences_speaker.py:49

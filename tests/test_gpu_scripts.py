@@ -118,3 +118,18 @@ def test_train_wavernn_cadence(tmp_path):
     assert int(torch.load(ck / 'latest_weights.pyt', map_location='cpu', weights_only=True)['step']) == 6
     run(*common, '--total_steps', '8')
     assert int(torch.load(ck / 'latest_weights.pyt', map_location='cpu', weights_only=True)['step']) == 9
+
+
+def test_synthesize_a_file_of_sentences_with_the_autoregressive_model(tmp_path):
+    """scripts/synthesize_sentences.py --model autoregressive --text-file: the sentences decode side by side, --in-flight at a time, and the
+    waveforms come out under the sentences' numbers."""
+    text = 'D@ kwIk braUn fQks dZVmps oUv@ D@ leIzi dQg'
+    (tmp_path / 'sentences.txt').write_text('\n'.join([text, text[:20], '', text[5:]]) + '\n')
+    np.save(tmp_path / 'spk.npy', np.random.default_rng(1).normal(size=256).astype(np.float32))
+    log = run('scripts/synthesize_sentences.py', '--config', 'config/wavernn', '--model', 'autoregressive', '--text-file', str(tmp_path / 'sentences.txt'),
+              '--spk-embed', str(tmp_path / 'spk.npy'), '--max-length', '59', '--in-flight', '2', '--out', str(tmp_path / 'wav.npy'))
+    assert '3 sentences, 2 in flight' in log
+    for i in range(3):
+        wav = np.load(tmp_path / f'wav_{i}.npy')
+        assert wav.ndim == 1 and len(wav) > 1000 and np.isfinite(wav).all()
+    assert not (tmp_path / 'wav_3.npy').exists()
