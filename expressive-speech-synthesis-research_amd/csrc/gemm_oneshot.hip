@@ -185,8 +185,8 @@ __global__ __launch_bounds__(NW * 64) void gemm_oneshot_kernel(const estts_gemm_
 // first reduction; the workgroups of column tile 0 also write their own rows (not the halo) to ln_out.
 #ifdef ESTTS_ONESHOT_STAMPS
 // Diagnostic build (-DESTTS_ONESHOT_STAMPS, tools/oneshot_stamps.py): lane 0 of wave 0 of every workgroup of the convolution
-// kernel leaves the 100 MHz clock at its phase boundaries.  The marks cost registers (122 -> 139 at 600 x 512 x 768 with the
-// LayerNorm prologue, i.e. one workgroup per CU instead of two), so the kernel under test is not quite the shipped one.
+// kernel leaves the 100 MHz clock at its phase boundaries.  The marks cost registers (120 -> 121 at 600 x 512 x 768 with the
+// LayerNorm prologue: still two workgroups per CU).
 __device__ unsigned long long oneshot_stamps[1024][8];
 #define OS_STAMP(i) do { if (threadIdx.x == 0) oneshot_stamps[(blockIdx.x + gridDim.x * blockIdx.y) & 1023][i] = wall_clock64(); } while (0)
 }  // namespace
@@ -237,25 +237,30 @@ __global__ __launch_bounds__(NW * 64) void gemm_oneshot_conv_kernel(const estts_
         }
     }
 
-    // ---- epilogue operands
+    // ---- epilogue operands: requested up front, or, behind a LayerNorm prologue, once the rows are staged; they then land during the
+    // products.  A prologue's rows and reductions leave no registers for them: at 600 x 512 x 768, where 304 workgroups want two per
+    // CU (at most 128 registers), up front / late: 136 / 120 registers, 13.7 / 11.3 us.
     float e_s1[OUTS], e_b1[OUTS], e_s2[OUTS], e_b2[OUTS], e_r[OUTS];
     int e_row[OUTS], e_col[OUTS];
     bool e_ok[OUTS];
+    auto request_epilogue = [&]() {
 #pragma unroll
-    for (int o = 0; o < OUTS; ++o) {
-        const int f = wave + o * NW;
-        const int i = f / (4 * T), j = (f >> 2) % T, r = f & 3;
-        e_row[o] = m0 + i * 16 + g * 4 + r;
-        e_col[o] = n0 + j * 16 + i16;
-        e_ok[o] = f < NF && e_row[o] < p.M && e_col[o] < p.N;
-        const int col = e_ok[o] ? e_col[o] : 0;
-        const int row = e_ok[o] ? e_row[o] : 0;
-        e_s1[o] = p.s1 ? p.s1[col] : 1.0f;
-        e_b1[o] = p.b1 ? p.b1[col] : 0.0f;
-        e_s2[o] = p.s2 ? p.s2[col] : 1.0f;
-        e_b2[o] = p.s2 ? p.b2[col] : 0.0f;
-        e_r[o] = p.R ? p.R[(long)(p.r_mod > 0 ? row % p.r_mod : row) * p.ldr + col] : 0.0f;
-    }
+        for (int o = 0; o < OUTS; ++o) {
+            const int f = wave + o * NW;
+            const int i = f / (4 * T), j = (f >> 2) % T, r = f & 3;
+            e_row[o] = m0 + i * 16 + g * 4 + r;
+            e_col[o] = n0 + j * 16 + i16;
+            e_ok[o] = f < NF && e_row[o] < p.M && e_col[o] < p.N;
+            const int col = e_ok[o] ? e_col[o] : 0;
+            const int row = e_ok[o] ? e_row[o] : 0;
+            e_s1[o] = p.s1 ? p.s1[col] : 1.0f;
+            e_b1[o] = p.b1 ? p.b1[col] : 0.0f;
+            e_s2[o] = p.s2 ? p.s2[col] : 1.0f;
+            e_b2[o] = p.s2 ? p.b2[col] : 0.0f;
+            e_r[o] = p.R ? p.R[(long)(p.r_mod > 0 ? row % p.r_mod : row) * p.ldr + col] : 0.0f;
+        }
+    };
+    if constexpr (LNCH == 0) request_epilogue();
 
     // ---- stage source rows m0 - lpad .. + rows_staged - 1 (clamped into the buffer; validity is decided at use)
     if constexpr (LNCH == 0) {
@@ -392,6 +397,7 @@ __global__ __launch_bounds__(NW * 64) void gemm_oneshot_conv_kernel(const estts_
             }
         }
     }
+    if constexpr (LNCH > 0) request_epilogue();
     OS_STAMP(2);
     __syncthreads();
     OS_STAMP(3);
