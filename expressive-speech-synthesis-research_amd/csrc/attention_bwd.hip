@@ -78,8 +78,10 @@ __global__ __launch_bounds__(256) void attention_delta_kernel(const estts_attent
     }
 }
 
+// (three workgroups per CU for the dQ pass at depth 64, split operands, which takes 172 registers left alone, one step above what they
+// need, and 162 without a spill where it is told: 8 x 4 heads x 272 x 272, both passes 35.6 -> 33.1 us, 4 x 4 x 600 x 600 56.0 -> 52.7)
 template <int DH, int NS, bool OWN_Q>
-__global__ __launch_bounds__(256) void attention_bwd_kernel(const estts_attention_bwd_args p) {
+__global__ __launch_bounds__(256, (DH == 64 && NS == 2 && OWN_Q ? 3 : 1)) void attention_bwd_kernel(const estts_attention_bwd_args p) {
     constexpr int KS = DH / 32;
     constexpr int NT = DH / 16;
     constexpr int LD = DH + 8;
@@ -264,10 +266,11 @@ __global__ __launch_bounds__(256) void attention_bwd_kernel(const estts_attentio
 // tile is fetched from L2 and split once per 64 owned rows instead of once per 16: at batch 32 the kernel above is bound
 // by exactly that traffic.  Every wave keeps the whole sum of its own rows, so nothing is merged at the end.  The weights
 // and delta of the next tile are fetched together with its rows, one tile ahead of their use.
-// workgroups per CU the register budget must allow (depth 64, split operands: the dQ pass compiles to 132 registers and the
-// dK / dV pass to 176 left alone, each one step above an occupancy threshold)
+// workgroups per CU the register budget must allow (split operands: at depth 64 the dQ pass compiles to 132 registers and the dK / dV pass
+// to 176 left alone, at depth 32 the dK / dV pass to 132, each one step above an occupancy threshold; the last, both passes: 32 x 4 heads x
+// 600 x 600 107.8 -> 102.1 us, 16 x 8 x 400 x 400 60.7 -> 57.7)
 template <int DH, int NS, bool OWN_Q>
-constexpr int bwd_wide_occupancy() { return (DH == 64 && NS == 2) ? (OWN_Q ? 4 : 3) : 1; }
+constexpr int bwd_wide_occupancy() { return NS == 2 ? (DH == 64 ? (OWN_Q ? 4 : 3) : DH == 32 ? 4 : 1) : 1; }
 
 template <int DH, int NS, bool OWN_Q>
 __global__ __launch_bounds__(256, (bwd_wide_occupancy<DH, NS, OWN_Q>())) void attention_bwd_wide_kernel(const estts_attention_bwd_args p) {

@@ -75,3 +75,14 @@ def test_convolutions_behind_a_norm_leave_room_for_two_workgroups_per_cu(tmp_pat
         pytest.skip('no objects under csrc/ (they are built by __graft_entry__.build())')
     found = [k for k in kernels_of(obj, str(tmp_path)) if 'gemm_oneshot_conv_kernel' + name in k[0]]
     assert len(found) == 1 and found[0][2] <= 128 and found[0][1] == 0, found
+
+
+@pytest.mark.skipif(not all(os.path.exists(t) for t in TOOLS), reason='LLVM binary tools not found')
+@pytest.mark.parametrize('name,most', [('attention_bwd_kernelILi64ELi2ELb1E', 168), ('attention_bwd_wide_kernelILi32ELi2ELb0E', 128)])
+def test_backward_passes_keep_their_workgroups_per_cu(tmp_path, name, most):
+    """Three workgroups of four waves up to 168 registers, four up to 128."""
+    obj = os.path.join(CSRC, 'attention_bwd.o')
+    if not os.path.exists(obj):
+        pytest.skip('no objects under csrc/ (they are built by __graft_entry__.build())')
+    found = [k for k in kernels_of(obj, str(tmp_path)) if name in k[0]]
+    assert len(found) == 1 and found[0][2] <= most and found[0][1] == 0, found
