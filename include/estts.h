@@ -948,7 +948,8 @@ int estts_page_write(const estts_page_write_args* args, void* stream);
  * positions a request: any value but 0 leaves the row out, whatever the row holds, as rows behind the length are left out
  * (estts_attention adds -1e9 instead, so that a fully masked row there is a mean of the values).  The rows that count and the
  * queries are finite (an infinity among them may come out as NaN).  max_len bounds the lengths (0: P page); it decides how the work is split, and a low bound lets short
- * requests run in one launch.  Products and sums have float32 accuracy for every cache type.
+ * requests run in one launch.  Sums are float32 for every cache type, and so are products, except that 16-bit pages
+ * which several query heads read are multiplied exactly by queries and weights held in 24 bits (bfloat16 pages) or 22 bits (float16 pages).
  * ws: estts_paged_attention_ws_bytes() bytes (may be NULL where that is 0) that belong to this call until it has run. */
 typedef struct estts_paged_attention_args {
     const float* q; int64_t ldq;
