@@ -646,6 +646,13 @@ def _check_here(what, names, *tensors):
     raise ValueError(f'{what}: {names.split()[i]} is on {tensors[i].device}, which is not the current device')
 
 
+def _check_sizes(what, **sizes):
+    """Sizes that the C ABI takes as int32, into which ctypes would cut larger ones without a word."""
+    for name, n in sizes.items():
+        if not -2 ** 31 <= n < 2 ** 31:
+            raise ValueError(f'{what}: {name} must stay below 2**31, got {n}')
+
+
 def _check_rows(what, t, name, rows, width):
     """Row stride of a [rows, >= width] float32 view with contiguous rows."""
     if t.dtype is not torch.float32:
@@ -733,6 +740,7 @@ def page_plan(lengths, new, block_table, free_pages, n_free, page, slots, positi
     P, ld = _check_table('page_plan', block_table, B)
     if slots.dim() != 1 and not (padded and slots.shape[0] == B):
         raise ValueError(f'page_plan: slots must be [T] (packed rows) or [{B}, R] (padded rows), got {list(slots.shape)}')
+    _check_sizes('page_plan', requests=B, rows=T, pages_of_a_request=P, pages=free_pages.numel(), page=page)
     _check_here('page_plan', 'lengths new block_table free_pages n_free slots positions lengths_out n_free_out refused', lengths, new, block_table,
                 free_pages, n_free, slots, positions, lengths_out, n_free_out, refused)
     lib = _lib.load()
@@ -764,6 +772,7 @@ def page_write(k, v, k_cache, v_cache, slots):
     T = slots.numel()
     _check_i32('page_write', slots, 'slots', slots.shape)
     ldk, ldv = _check_rows('page_write', k, 'k', T, Hk * D), _check_rows('page_write', v, 'v', T, Hk * D)
+    _check_sizes('page_write', rows=T, pages=n_pages, heads=Hk, page=page, depth=D)
     _check_here('page_write', 'k v k_cache v_cache slots', k, v, k_cache, v_cache, slots)
     a = _lib.PageWriteArgs(k.data_ptr(), ldk, v.data_ptr(), ldv, k_cache.data_ptr(), v_cache.data_ptr(), s_page, s_head, s_row, slots.data_ptr(),
                            T, Hk, D, page, n_pages, KV_TYPES[k_cache.dtype])
@@ -783,7 +792,8 @@ def paged_attention(q, k_cache, v_cache, block_table, lengths, ctx, heads, key_m
     memory), heads a multiple of kv_heads: query head h reads key head h // (heads / kv_heads); block_table [B, P], lengths [B] int32 as
     page_plan leaves them (the new row is in its page already).  key_mask: [B, >= max_len] float32 view, rows with any value but 0 are
     left out; a request with nothing left gets zeros.  scale: 1 / sqrt(depth) if None.  max_len: bound on the lengths that the host
-    knows of (P * page if None; rows past it are not read)."""
+    knows of (P * page if None; rows past it are not read); in a StepProgram the bound for all of its steps, since the scratch of a call goes
+    by it."""
     host = _issue()
     if host is not None and host.paged_attention(q, k_cache, v_cache, block_table, lengths, ctx, heads, key_mask, scale, max_len):
         return ctx
@@ -805,6 +815,7 @@ def paged_attention(q, k_cache, v_cache, block_table, lengths, ctx, heads, key_m
         if key_mask.dim() != 2 or key_mask.shape[0] != B or key_mask.shape[1] < max_len:
             raise ValueError(f'paged_attention: key_mask must be [{B}, >= {max_len}], got {list(key_mask.shape)}')
         sb, ss = key_mask.stride()
+    _check_sizes('paged_attention', requests=B, pages_of_a_request=P, pages=n_pages, heads=heads, page=page, depth=D, max_len=max_len)
     _check_here('paged_attention', 'q k_cache v_cache block_table lengths ctx key_mask', q, k_cache, v_cache, block_table, lengths, ctx, key_mask)
     lib, kind = _lib.load(), KV_TYPES[k_cache.dtype]
     nbytes = lib.estts_paged_attention_ws_bytes(B, heads, Hk, D, max_len, kind)

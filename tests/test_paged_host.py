@@ -393,3 +393,26 @@ def test_without_a_usable_cpp_module_calls_take_the_python_path(monkeypatch, tmp
         assert ops._issue() is None and _lib._host is False
         with pytest.raises((ValueError, TypeError)):                # (the Python path, and its checks)
             ops.paged_attention(*[torch.zeros(1)] * 6, 1)
+
+
+# ------------------------------------------------------------------------------------------------- sizes that do not fit 32 bits
+def meta(*shape, dtype=torch.int32):
+    return torch.empty(*shape, dtype=dtype, device='meta')
+
+
+@pytest.mark.parametrize('name,call', [
+    ('rows', lambda: ops.page_plan(meta(3), meta(3), meta(3, 8), meta(32), meta(1), 16, meta(2 ** 32 + 5))),
+    ('pages', lambda: ops.page_plan(meta(3), meta(3), meta(3, 8), meta(2 ** 32 + 5), meta(1), 16, meta(4))),
+    ('requests', lambda: ops.page_plan(meta(2 ** 32 + 3), meta(2 ** 32 + 3), meta(2 ** 32 + 3, 8), meta(32), meta(1), 16, meta(4))),
+    ('pages_of_a_request', lambda: ops.page_plan(meta(3), meta(3), meta(3, 2 ** 32 + 8), meta(32), meta(1), 16, meta(4))),
+    ('page', lambda: ops.page_plan(meta(3), meta(3), meta(3, 8), meta(32), meta(1), 2 ** 32 + 16, meta(4))),
+    ('rows', lambda: ops.page_write(*[meta(2 ** 32 + 5, 64, dtype=torch.float32)] * 2, *[meta(4, 2, 16, 32, dtype=torch.float32)] * 2, meta(2 ** 32 + 5))),
+    ('pages', lambda: ops.page_write(*[meta(5, 64, dtype=torch.float32)] * 2, *[meta(2 ** 32 + 4, 2, 16, 32, dtype=torch.float32)] * 2, meta(5))),
+    ('requests', lambda: ops.paged_attention(meta(2 ** 32 + 1, 64, dtype=torch.float32), *[meta(4, 2, 16, 32, dtype=torch.float32)] * 2, meta(2 ** 32 + 1, 8),
+                                             meta(2 ** 32 + 1), meta(2 ** 32 + 1, 64, dtype=torch.float32), 2, max_len=64)),
+    ('pages_of_a_request', lambda: ops.paged_attention(meta(1, 64, dtype=torch.float32), *[meta(4, 2, 16, 32, dtype=torch.float32)] * 2, meta(1, 2 ** 32 + 1),
+                                                       meta(1), meta(1, 64, dtype=torch.float32), 2, max_len=64))])
+def test_sizes_past_32_bits_are_refused(name, call):
+    """As int32 fields of the argument block 2**32 + 5 rows would be five: the plan of the others would stay as it was."""
+    with pytest.raises(ValueError, match=rf': {name} must stay below 2\*\*31'):
+        call()
